@@ -1,0 +1,103 @@
+// bx_ops.h -- what the dense operators over keypoints share (k_linear.hip, k_rope.hip, k_attn.hip): element types, 16-byte chunks and the
+// matrix instructions that consume them.  A chunk is 16 bytes of one row: 4 floats or 8 halves.  Every kernel feeds the matrix units
+// one chunk per lane and operand, so the three element types share one code path:
+//   f16 / bf16: one v_mfma_f32_32x32x16 (16x16x32) per chunk;
+//   f32:        four v_mfma_f32_32x32x2 (16x16x4), step j taking element j of both operands' chunks -- the products of a sum are
+//               visited in another order than by k, the same one on both sides.
+#pragma once
+#include "bx_common.h"
+
+typedef float bxf4 __attribute__((ext_vector_type(4)));
+typedef float bxf16 __attribute__((ext_vector_type(16)));
+typedef int bxi4 __attribute__((ext_vector_type(4)));
+typedef int bxi2 __attribute__((ext_vector_type(2)));
+typedef _Float16 bxh8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bxb8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bx_bf16;
+typedef _Float16 bx_f16;
+
+// 16 bytes at any element boundary (gfx950 loads and stores them unaligned in one instruction)
+struct __attribute__((packed, aligned(2))) BxAny16 { bxi4 v; };
+
+template <class T> struct BxElem {
+    static constexpr int CH = 16 / (int)sizeof(T);      // elements per chunk
+};
+
+template <class T> __device__ __forceinline__ bxf16 bx_mma32(bxi4 a, bxi4 b, bxf16 c)
+{
+    if constexpr (sizeof(T) == 4) {
+        const bxf4 x = __builtin_bit_cast(bxf4, a), y = __builtin_bit_cast(bxf4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, bx_f16)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(bxh8, a), __builtin_bit_cast(bxh8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bxb8, a), __builtin_bit_cast(bxb8, b), c, 0, 0, 0);
+    }
+}
+
+template <class T> __device__ __forceinline__ bxf4 bx_mma16(bxi4 a, bxi4 b, bxf4 c)
+{
+    if constexpr (sizeof(T) == 4) {
+        const bxf4 x = __builtin_bit_cast(bxf4, a), y = __builtin_bit_cast(bxf4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, bx_f16)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(bxh8, a), __builtin_bit_cast(bxh8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bxb8, a), __builtin_bit_cast(bxb8, b), c, 0, 0, 0);
+    }
+}
+
+// elements [k, k + CH) of a row of `n` elements as one chunk; what lies at or behind n is zero and is not read
+template <class T, bool ALIGNED> __device__ __forceinline__ bxi4 bx_load_chunk(const T* __restrict__ row, int k, int n)
+{
+    constexpr int CH = BxElem<T>::CH;
+    if (k + CH <= n) {
+        if constexpr (ALIGNED) return *reinterpret_cast<const bxi4*>(row + k);
+        else return reinterpret_cast<const BxAny16*>(row + k)->v;
+    }
+    T e[CH];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) e[j] = k + j < n ? row[k + j] : (T)0.0f;
+    bxi4 r;
+    __builtin_memcpy(&r, e, 16);
+    return r;
+}
+
+// four consecutive outputs of one row, rounded once to T (nearest, ties to even); `n` = how many of them exist
+template <class T, bool ALIGNED> __device__ __forceinline__ void bx_store4(T* __restrict__ p, const float* v, int n)
+{
+    T e[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = (T)v[j];
+    if (ALIGNED && n >= 4) {
+        if constexpr (sizeof(T) == 4) { bxi4 r; __builtin_memcpy(&r, e, 16); *reinterpret_cast<bxi4*>(p) = r; }
+        else { bxi2 r; __builtin_memcpy(&r, e, 8); *reinterpret_cast<bxi2*>(p) = r; }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < n) p[j] = e[j];
+}
+
+template <class T, bool ALIGNED> __device__ __forceinline__ void bx_load4(const T* __restrict__ p, float* v, int n)
+{
+    T e[4];
+    if (ALIGNED && n >= 4) {
+        if constexpr (sizeof(T) == 4) { const bxi4 r = *reinterpret_cast<const bxi4*>(p); __builtin_memcpy(e, &r, 16); }
+        else { const bxi2 r = *reinterpret_cast<const bxi2*>(p); __builtin_memcpy(e, &r, 8); }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = j < n ? p[j] : (T)0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (float)e[j];
+}
+
+int bxk_linear(hipStream_t s, int n_cu, const bx_linear_args& a);
+int bxk_qk_norm_rope(hipStream_t s, int n_cu, const bx_qk_norm_rope_args& a);
+int64_t bxk_attention_workspace(int n_cu, const bx_attention_args& a);
+int bxk_attention(hipStream_t s, int n_cu, const bx_attention_args& a);

@@ -52,6 +52,36 @@ class BxCapture(C.Structure):
                 ("T_ransac", C.c_void_p)]
 
 
+class BxLinearArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("act", C.c_int32), ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
+                ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldy", C.c_int64),
+                ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+                ("m_dev", C.c_void_p)]
+
+
+class BxQkNormRopeArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("norm", C.c_int32), ("pairs", C.c_int32), ("pos_dtype", C.c_int32), ("T", C.c_int64),
+                ("Hq", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32), ("axes", C.c_int32), ("sections", C.c_int32 * 4),
+                ("eps", C.c_float), ("reserved", C.c_int32),
+                ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+                ("q_out_stride_t", C.c_int64), ("q_out_stride_h", C.c_int64), ("k_out_stride_t", C.c_int64),
+                ("k_out_stride_h", C.c_int64), ("pos_stride_t", C.c_int64),
+                ("q", C.c_void_p), ("k", C.c_void_p), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("pos", C.c_void_p),
+                ("freqs", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("m_dev", C.c_void_p)]
+
+
+class BxAttentionArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("Lq", C.c_int32), ("Lk", C.c_int32), ("Hq", C.c_int32), ("Hk", C.c_int32),
+                ("D", C.c_int32), ("left", C.c_int32), ("right", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float),
+                ("reserved", C.c_int32),
+                ("q_stride_b", C.c_int64), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64),
+                ("k_stride_b", C.c_int64), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+                ("v_stride_b", C.c_int64), ("v_stride_t", C.c_int64), ("v_stride_h", C.c_int64),
+                ("o_stride_b", C.c_int64), ("o_stride_t", C.c_int64), ("o_stride_h", C.c_int64),
+                ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("q_lens", C.c_void_p),
+                ("k_lens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 EXPORTS = ["bx_create", "bx_destroy", "bx_last_error", "bx_load_weights", "bx_workspace_bytes", "bx_register_pair",
            "bx_register_pair_begin", "bx_register_pair_finish",
            "bx_set_capture", "bx_keypoint_tile_bounds",
@@ -60,6 +90,7 @@ EXPORTS = ["bx_create", "bx_destroy", "bx_last_error", "bx_load_weights", "bx_wo
            "bx_desc_net", "bx_conv_layer",
            "bx_mutual", "bx_pose_net", "bx_hypotheses", "bx_consensus", "bx_ransac", "bx_kiss_solve", "bx_refine",
            "bx_pre_reserve", "bx_pre_voxel_downsample", "bx_pre_pca", "bx_random_perm",
+           "bx_linear", "bx_qk_norm_rope", "bx_attention_workspace", "bx_attention",
            "bx_lane_create", "bx_lane_destroy", "bx_attach_lane",
            "bx_io_probe", "bx_io_read_xyz", "bx_prefetch_create", "bx_prefetch_submit", "bx_prefetch_wait", "bx_prefetch_release",
            "bx_prefetch_destroy"]
@@ -88,6 +119,7 @@ def load():
         lib = C.CDLL(_SO)
         lib.bx_last_error.restype = C.c_char_p
         lib.bx_workspace_bytes.restype = C.c_int64
+        lib.bx_attention_workspace.restype = C.c_int64
         _LIB = lib
     return _LIB
 
@@ -191,6 +223,7 @@ class Context:
         self.lib = load()
         self.cfg = cfg
         self.device = device
+        self.tdevice = torch.device("cuda", device)
         self.params = params_from_cfg(cfg, max_points)
         self.handle = C.c_void_p()
         _chk(self.lib.bx_create(C.c_int(device), C.byref(self.params), C.byref(self.handle)), "bx_create")
@@ -332,6 +365,39 @@ class Context:
                                                 C.c_int32(P), self._p(radius_dev), C.c_int32(int(aligned)), self._p(R), self._p(feat)),
              "bx_patch_features_counted")
         return R, feat
+
+    # ---------------------------------------------------------------- dense operators over keypoints (dense.py: checks and layouts)
+    def linear(self, x, weight, bias=None, act="none", residual=None, out=None, m_dev=None):
+        """act(x @ weight.T + bias) + residual: x [M, K], weight [N, K], bias [N], residual / out [M, N] -> out.  act: "none",
+        "relu", "gelu", "silu".  m_dev: device int32 count of the rows in use (the others are left as they are in `out`)."""
+        from . import dense
+        args, out = dense.linear_args(self.torch, self.tdevice, x, weight, bias, act, residual, out, m_dev)
+        _chk(self.lib.bx_linear(self.handle, self._stream(), C.byref(args)), "bx_linear")
+        return out
+
+    def qk_norm_rope(self, q, k, pos, freqs, sections, norm="rms", eps=1e-6, q_weight=None, k_weight=None, pairs="half", q_out=None,
+                     k_out=None, m_dev=None):
+        """norm of every head of q [T, Hq, D] and k [T, Hk, D] (either may be None) and the rotation of sections[a] pairs by
+        pos[:, a] * freqs, in one pass -> (q_out, k_out).  norm: "none", "rms", "l2"; pairs: "half" ((p, p + P)) or "interleaved"
+        ((2 p, 2 p + 1)); pos [T, axes] float32 or int32; freqs float64 [sum(sections)].  q_out / k_out may be q / k."""
+        from . import dense
+        args, q_out, k_out = dense.qk_norm_rope_args(self.torch, self.tdevice, q, k, pos, freqs, sections, norm, eps, q_weight, k_weight, pairs,
+                                                     q_out, k_out, m_dev)
+        _chk(self.lib.bx_qk_norm_rope(self.handle, self._stream(), C.byref(args)), "bx_qk_norm_rope")
+        return q_out, k_out
+
+    def attention(self, q, k, v, scale=None, window=(-1, -1), sinks=0, q_lens=None, k_lens=None, out=None):
+        """attention of q [B, Lq, Hq, D] over k, v [B, Lk, Hk, D] -> [B, Lq, Hq, D].  window = (left, right): how many keys before and
+        behind its own position a query sees (-1: all; the last query stands at the last key); the first `sinks` keys stay visible
+        beyond `left`.  q_lens / k_lens: device int32 [B]; rows of `out` at or behind q_lens are left as they are."""
+        from . import dense
+        args, out = dense.attention_args(self.torch, self.tdevice, q, k, v, scale, window, sinks, q_lens, k_lens, out)
+        need = self.lib.bx_attention_workspace(self.handle, C.byref(args))
+        if need > 0:
+            ws = self.torch.empty(need, dtype=self.torch.uint8, device=self.tdevice)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), need
+        _chk(self.lib.bx_attention(self.handle, self._stream(), C.byref(args)), "bx_attention")
+        return out
 
     # ---------------------------------------------------------------- pre-processing (SURVEY §8f rank 1)
     def pre_reserve(self, max_points):

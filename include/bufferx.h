@@ -301,6 +301,92 @@ int bx_kiss_solve(bx_ctx *ctx, void *stream, const float *ss, const float *tt, c
 int bx_refine(bx_ctx *ctx, void *stream, const float *ss, const float *tt, const int32_t *M_dev, int32_t max_M,
               float *T_io, int32_t *iters_out);
 
+/* ---- dense operators over keypoints (no reference counterpart) --------------------------------------------------------------
+ * The parts of a layer that lets the descriptors of two clouds see each other between bx_desc_net and bx_mutual: a dense layer, the
+ * norm of queries and keys with a rotation by position, and attention.  Inference only, as everything here: there is no backward pass.
+ *
+ * Types: BX_TYPE_* of every operand that is not stated otherwise (float32, IEEE half, bfloat16).  Sums, norms and softmax statistics
+ * are held in float32, angles in binary64; every output is rounded once.  Inputs are read through element strides (the innermost
+ * dimension is contiguous; a stride of 0 repeats a row), any element alignment is accepted and 16-byte aligned rows are faster.
+ * Counts and lengths that depend on the data are device int32, read when the kernel runs and clamped to [0, the size given here];
+ * rows at or behind them are neither read nor written.  Sizes of zero are answered without a launch.
+ * Outputs must not overlap any input (exceptions are named) nor themselves: BX_ERR_ARG.  Results do not depend on the stream, on the
+ * run or on other calls: the order of every sum is fixed by the sizes.  The calls keep no state and share none, so several may run at
+ * once, on one context too, and may be captured; the memory they are given must stay valid until they have run.  */
+#define BX_TYPE_F32 0
+#define BX_TYPE_F16 1
+#define BX_TYPE_BF16 2
+#define BX_ACT_NONE 0
+#define BX_ACT_RELU 1
+#define BX_ACT_GELU 2    /* v Phi(v), Phi the normal distribution function (the exact form) */
+#define BX_ACT_SILU 3    /* v / (1 + exp(-v)) */
+
+/* y = act(x w^T + bias) + residual.  x [M][K], w [N][K], bias [N] (nullable), residual and y [M][N] (residual nullable; it may be y
+ * itself, with the same stride).  M, N, K < 2^31.  m_dev (nullable): device count of the rows that are in use.            */
+typedef struct bx_linear_args {
+    int32_t dtype, act;
+    int64_t M, N, K;
+    int64_t ldx, ldw, ldr, ldy;      /* elements between rows */
+    const void *x, *w, *bias, *residual;
+    void *y;
+    const int32_t *m_dev;
+} bx_linear_args;
+int bx_linear(bx_ctx *ctx, void *stream, const bx_linear_args *args);
+
+/* q [T][Hq][D] and k [T][Hk][D] (either pointer nullable), every head row x of length D (1..256):
+ *   y = x * w * n,   n = 1 (BX_NORM_NONE), 1 / sqrt(mean(x^2) + eps) (BX_NORM_RMS), 1 / max(|x|, eps) (BX_NORM_L2); w [D] nullable = 1
+ *   then rotation pair p of axis a:  (y_i, y_j) -> (y_i cos t - y_j sin t, y_j cos t + y_i sin t),  t = pos[token][a] * freqs[p].
+ * sections[a] = number of pairs of axis a (axes 1..4; the pairs of axis 0 come first, P = their sum, 2 P <= D); (i, j) = (p, p + P)
+ * with BX_PAIRS_HALF, (2 p, 2 p + 1) with BX_PAIRS_INTERLEAVED; elements from 2 P on are not rotated.
+ * pos [T][axes] float32 or int32, freqs float64 [P] (radians per unit of position).  m_dev (nullable): device count of the tokens
+ * in use.  q_out may be q itself and k_out k itself (same strides); interleaved rows of one buffer are not an overlap. */
+#define BX_NORM_NONE 0
+#define BX_NORM_RMS 1
+#define BX_NORM_L2 2
+#define BX_PAIRS_HALF 0
+#define BX_PAIRS_INTERLEAVED 1
+#define BX_POS_F32 0
+#define BX_POS_I32 1
+typedef struct bx_qk_norm_rope_args {
+    int32_t dtype, norm, pairs, pos_dtype;
+    int64_t T;
+    int32_t Hq, Hk, D, axes;
+    int32_t sections[4];
+    float eps;
+    int32_t reserved;                /* 0 */
+    int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, q_out_stride_t, q_out_stride_h, k_out_stride_t, k_out_stride_h, pos_stride_t;
+    const void *q, *k, *q_weight, *k_weight, *pos;
+    const double *freqs;
+    void *q_out, *k_out;
+    const int32_t *m_dev;
+} bx_qk_norm_rope_args;
+int bx_qk_norm_rope(bx_ctx *ctx, void *stream, const bx_qk_norm_rope_args *args);
+
+/* Attention: q, o [B][Lq][Hq][D], k, v [B][Lk][Hk][D], Hq a multiple of Hk (query head h reads key head h / (Hq / Hk)), D 1..128.
+ *   o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys that query i of a batch entry sees:
+ *   j < k_len,  j <= p_i + right (right >= 0),  j >= p_i - left (left >= 0) or j < sinks,      p_i = i + k_len - q_len
+ * (the last query stands at the last key).  left / right < 0: no bound on that side.  A query that sees no key gets zeros; keys that it
+ * does not see do not touch its result, whatever they hold, infinities and NaN included.  scale > 0 and finite.
+ * q_lens / k_lens: device int32 [B], nullable (Lq / Lk).
+ * The softmax weights are rounded to the type of v before they are multiplied (f16 / bf16).
+ * workspace: device memory of bx_attention_workspace(ctx, args) bytes (0: none needed; a host function of the sizes alone), aligned to 16 bytes,
+ * used until the call has run and by no other call meanwhile; BX_ERR_STATE when it is too small.               */
+typedef struct bx_attention_args {
+    int32_t dtype, B, Lq, Lk, Hq, Hk, D;
+    int32_t left, right, sinks;
+    float scale;
+    int32_t reserved;                /* 0 */
+    int64_t q_stride_b, q_stride_t, q_stride_h, k_stride_b, k_stride_t, k_stride_h;
+    int64_t v_stride_b, v_stride_t, v_stride_h, o_stride_b, o_stride_t, o_stride_h;
+    const void *q, *k, *v;
+    void *o;
+    const int32_t *q_lens, *k_lens;
+    void *workspace;
+    int64_t workspace_bytes;
+} bx_attention_args;
+int64_t bx_attention_workspace(bx_ctx *ctx, const bx_attention_args *args);   /* < 0: bad argument */
+int bx_attention(bx_ctx *ctx, void *stream, const bx_attention_args *args);
+
 /* ---- lane: ordering of the pairs in flight on ONE GPU (optional) -----------------------------------------------------------
  * The reference runs one pair at a time (test.py:132-146).  Here several contexts / streams keep pairs in flight so that the
  * latency-bound furthest-point sampling of one pair overlaps the convolutions of another.  Contexts attached to the same lane
