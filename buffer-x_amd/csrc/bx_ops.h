@@ -67,34 +67,51 @@ template <class T, bool ALIGNED> __device__ __forceinline__ bxi4 bx_load_chunk(c
     return r;
 }
 
-// four consecutive outputs of one row, rounded once to T (nearest, ties to even); `n` = how many of them exist
-template <class T, bool ALIGNED> __device__ __forceinline__ void bx_store4(T* __restrict__ p, const float* v, int n)
+// four consecutive elements of one row, of which n exist.  Results are rounded once to T (nearest, ties to even).
+struct __attribute__((packed, aligned(2))) BxAny8 { bxi2 v; };
+template <class T> __device__ __forceinline__ void bx_store4(T* __restrict__ p, const float* v, int n)
 {
     T e[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) e[j] = (T)v[j];
-    if (ALIGNED && n >= 4) {
-        if constexpr (sizeof(T) == 4) { bxi4 r; __builtin_memcpy(&r, e, 16); *reinterpret_cast<bxi4*>(p) = r; }
-        else { bxi2 r; __builtin_memcpy(&r, e, 8); *reinterpret_cast<bxi2*>(p) = r; }
+    if (n >= 4) {
+        if constexpr (sizeof(T) == 4) { bxi4 r; __builtin_memcpy(&r, e, 16); reinterpret_cast<BxAny16*>(p)->v = r; }
+        else { bxi2 r; __builtin_memcpy(&r, e, 8); reinterpret_cast<BxAny8*>(p)->v = r; }
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 3; ++j)
         if (j < n) p[j] = e[j];
 }
 
-template <class T, bool ALIGNED> __device__ __forceinline__ void bx_load4(const T* __restrict__ p, float* v, int n)
+template <class T> __device__ __forceinline__ void bx_load4(const T* __restrict__ p, float* v, int n)
 {
     T e[4];
-    if (ALIGNED && n >= 4) {
-        if constexpr (sizeof(T) == 4) { const bxi4 r = *reinterpret_cast<const bxi4*>(p); __builtin_memcpy(e, &r, 16); }
-        else { const bxi2 r = *reinterpret_cast<const bxi2*>(p); __builtin_memcpy(e, &r, 8); }
+    if (n >= 4) {
+        if constexpr (sizeof(T) == 4) { const bxi4 r = reinterpret_cast<const BxAny16*>(p)->v; __builtin_memcpy(e, &r, 16); }
+        else { const bxi2 r = reinterpret_cast<const BxAny8*>(p)->v; __builtin_memcpy(e, &r, 8); }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] = j < n ? p[j] : (T)0.0f;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = (float)e[j];
+}
+
+// 16 bytes per lane from memory straight into LDS, at lds + 16 lane (lds is the same for the whole wave)
+__device__ __forceinline__ void bx_load_lds16(const void* g, void* lds)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+// Workgroups go to the eight XCDs in turn.  This order gives each XCD runs of C neighbours of the logical order instead, whose operands
+// its L2 then reads once; what does not fill whole rounds keeps its place.
+template <unsigned C> __device__ __forceinline__ unsigned bx_xcd_order(unsigned id, unsigned n)
+{
+    const unsigned full = n / (8 * C) * (8 * C);
+    if (id >= full) return id;
+    const unsigned x = id & 7, j = id >> 3;
+    return j / C * (8 * C) + x * C + j % C;
 }
 
 int bxk_linear(hipStream_t s, int n_cu, const bx_linear_args& a);

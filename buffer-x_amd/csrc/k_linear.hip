@@ -22,21 +22,21 @@ struct LinearK {
     int M, N, K, act, tiles_n;
 };
 
-template <class T, bool ALIGNED>
+template <class T>
 __device__ __forceinline__ void epilogue4(const LinearK& p, int m, int n, const float* acc)
 {
     const int left = p.N - n;
     float v[4], b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.bias) bx_load4<T, ALIGNED>((const T*)p.bias + n, b, left);
+    if (p.bias) bx_load4<T>((const T*)p.bias + n, b, left);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = act_of(acc[j] + b[j], p.act);
     if (p.residual) {
         float r[4];
-        bx_load4<T, ALIGNED>((const T*)p.residual + (long long)m * p.ldr + n, r, left);
+        bx_load4<T>((const T*)p.residual + (long long)m * p.ldr + n, r, left);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += r[j];
     }
-    bx_store4<T, ALIGNED>((T*)p.y + (long long)m * p.ldy + n, v, left);
+    bx_store4<T>((T*)p.y + (long long)m * p.ldy + n, v, left);
 }
 
 // One workgroup = a BM x BN tile of y; a wave holds a (BM / WGM) x (BN / WGN) part of it in 32 x 32 accumulators.  The matrix product is
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void linear_tile_kernel(LinearK p)
                 const int n = n0 + wn + a * 32 + 8 * g + 4 * h;
                 if (n >= p.N) continue;
                 const float v[4] = {acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
-                epilogue4<T, ALIGNED>(p, m, n, v);
+                epilogue4<T>(p, m, n, v);
             }
     }
 }
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(LinearK p)
         for (int w = 0; w < NW; ++w)
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += part[w][lr][4 * q + i];
-        if (m < M && n < p.N) epilogue4<T, ALIGNED>(p, m, n, v);
+        if (m < M && n < p.N) epilogue4<T>(p, m, n, v);
     }
 }
 
@@ -185,8 +185,7 @@ int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
 {
     LinearK k = {a.x, a.w, a.bias, a.residual, a.y, a.m_dev, a.ldx, a.ldw, a.ldr, a.ldy, (int)a.M, (int)a.N, (int)a.K, a.act, 0};
     const auto al16 = [](const void* p, long long ld) { return ((uintptr_t)p & 15) == 0 && (ld * (long long)sizeof(T)) % 16 == 0; };
-    const bool aligned = al16(a.x, a.ldx) && al16(a.w, a.ldw) && al16(a.y, a.ldy) && (!a.residual || al16(a.residual, a.ldr)) &&
-                         (!a.bias || al16(a.bias, 0));
+    const bool aligned = al16(a.x, a.ldx) && al16(a.w, a.ldw);
     const long long tiles64 = (long long)((k.M + 63) / 64) * ((k.N + 63) / 64);
     if (k.M <= 32 || (tiles64 < n_cu / 2 && k.K >= 256)) {
         k.tiles_n = (k.N + 15) / 16;
