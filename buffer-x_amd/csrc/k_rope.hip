@@ -43,66 +43,185 @@ __device__ __forceinline__ void sincos64(double x, float& s, float& c)
     c = (float)(((m + 1) & 2) ? -co : co);
 }
 
-constexpr int ROPE_PAIRS = 128;      // rotation pairs of a head (D <= 256)
-
-// One workgroup = one token: its angles once for all heads into LDS, then a wave per head.
-template <class T>
-__global__ __launch_bounds__(256) void rope_kernel(RopeK p)
+// N consecutive elements (16 bytes), of which n exist
+template <class T, int N, bool VEC> __device__ __forceinline__ bxi4 load_piece(const T* p, int n)
 {
-    __shared__ float sc[ROPE_PAIRS], ss[ROPE_PAIRS];
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (p.m_dev && t >= *p.m_dev) return;
-    for (int i = tid; i < p.pairs; i += 256) {
+    bxi4 r = {0, 0, 0, 0};
+    if constexpr (VEC) {
+        if (n > 0) r = *reinterpret_cast<const bxi4*>(p);
+    } else {
+        T e[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) e[j] = j < n ? p[j] : (T)0.0f;
+        __builtin_memcpy(&r, e, 16);
+    }
+    return r;
+}
+template <class T, int N> __device__ __forceinline__ void floats_of(bxi4 r, float* v)
+{
+    T e[N];
+    __builtin_memcpy(e, &r, 16);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (float)e[j];
+}
+template <class T, int N, bool VEC> __device__ __forceinline__ void store_piece(T* p, const float* v, int n)
+{
+    T e[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) e[j] = (T)v[j];
+    if constexpr (VEC) {
+        bxi4 r;
+        __builtin_memcpy(&r, e, 16);
+        if (n > 0) *reinterpret_cast<bxi4*>(p) = r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < n) p[j] = e[j];
+    }
+}
+
+// A workgroup serves TPB tokens.  Their angles are formed once for all heads into LDS; then LPR lanes take a head row, N = 8 or 4
+// elements of its first stretch and as many of its second stretch each, so that both ends of a rotation pair are in one lane:
+//   HALF:        elements [N x, N x + N) and [P + N x, P + N x + N)  -- the pairs N x ..
+//   interleaved: elements [2 N x, 2 N x + 2 N)                       -- the pairs N x ..
+// What lies behind 2 P is a row of its own kind: plain elements, 2 N a lane.  VEC: the pieces are read and written whole (P and D are
+// multiples of N, and of 2 N where they are not rotated); otherwise element by element, with the same arrangement.
+template <class T, int LPR, int N, bool HALF, bool VEC>
+__global__ __launch_bounds__(256) void rope_kernel(RopeK p, int tpb)
+{
+    extern __shared__ float angles[];                        // [tpb][P] cos, then sin
+    constexpr int RPB = 256 / LPR;
+    const int tid = threadIdx.x, P = p.pairs;
+    int T_ = p.T;
+    if (p.m_dev) { const int live = *p.m_dev; T_ = live < T_ ? live : T_; }
+    const int t0 = (int)blockIdx.x * tpb;
+    if (t0 >= T_) return;
+    const int nt = min(tpb, T_ - t0);
+    const int x = tid % LPR, H = p.Hq + p.Hk;
+    // this lane's elements: two pieces of N
+    const bool turn = N * x < P;
+    const int u = 2 * N * x, tail = 2 * P;                   // interleaved, or behind the pairs
+    const int px = (P + N - 1) / N;                          // lanes that hold pairs
+    const int e0 = turn ? (HALF ? N * x : u) : tail + 2 * N * (x - px), e1 = turn && HALF ? P + N * x : e0 + N;
+    // how many of each piece exist
+    const int n0 = turn ? (HALF ? min(N, P - N * x) : min(N, 2 * P - e0)) : max(0, min(N, p.D - e0));
+    const int n1 = turn ? (HALF ? n0 : max(0, min(N, 2 * P - e1))) : max(0, min(N, p.D - e1));
+    // a row's elements are on their way while the angles, or the row before, are worked out
+    bxi4 ra, rb;
+    const auto fetch = [&](int row) {
+        const int t = row / H, hh = row - t * H;
+        const long long tok = t0 + t;
+        const T* in = hh < p.Hq ? (const T*)p.q + tok * p.qs_t + (long long)hh * p.qs_h : (const T*)p.k + tok * p.ks_t + (long long)(hh - p.Hq) * p.ks_h;
+        ra = load_piece<T, N, VEC>(in + e0, n0);
+        rb = load_piece<T, N, VEC>(in + e1, n1);
+    };
+    if (tid / LPR < nt * H) fetch(tid / LPR);
+    float *cs = angles, *sn = angles + tpb * P;
+    for (int i = tid; i < nt * P; i += 256) {
+        const int t = i / P, pr = i - t * P;
         int ax = 0, e = p.sec[0];
-        while (i >= e && ax + 1 < p.axes) e += p.sec[++ax];
-        const double at = p.pos_int ? (double)((const int32_t*)p.pos)[(long long)t * p.pos_t + ax] : (double)((const float*)p.pos)[(long long)t * p.pos_t + ax];
-        sincos64(at * p.freqs[i], ss[i], sc[i]);
+        while (pr >= e && ax + 1 < p.axes) e += p.sec[++ax];
+        const long long at = (long long)(t0 + t) * p.pos_t + ax;
+        const double pos = p.pos_int ? (double)((const int32_t*)p.pos)[at] : (double)((const float*)p.pos)[at];
+        sincos64(pos * p.freqs[pr], sn[i], cs[i]);
     }
     __syncthreads();
-    for (int hh = wave; hh < p.Hq + p.Hk; hh += 4) {
+    for (int row = tid / LPR; row < nt * H; row += RPB) {
+        const int t = row / H, hh = row - t * H;
         const bool isq = hh < p.Hq;
-        const int hd = isq ? hh : hh - p.Hq;
-        const T* x = isq ? (const T*)p.q + (long long)t * p.qs_t + (long long)hd * p.qs_h : (const T*)p.k + (long long)t * p.ks_t + (long long)hd * p.ks_h;
-        T* y = isq ? (T*)p.qo + (long long)t * p.qos_t + (long long)hd * p.qos_h : (T*)p.ko + (long long)t * p.kos_t + (long long)hd * p.kos_h;
+        const long long tok = t0 + t;
+        T* out = isq ? (T*)p.qo + tok * p.qos_t + (long long)hh * p.qos_h : (T*)p.ko + tok * p.kos_t + (long long)(hh - p.Hq) * p.kos_h;
         const T* w = (const T*)(isq ? p.qw : p.kw);
-        // lane holds pairs lane and lane + 64, and the unrotated elements behind the pairs the same way
-        float a[2], b[2], u[4];
-        int ia[2], ib[2];
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int pr = lane + 64 * i;
-            ia[i] = p.half ? pr : 2 * pr;
-            ib[i] = p.half ? pr + p.pairs : 2 * pr + 1;
-            a[i] = b[i] = 0.0f;
-            if (pr < p.pairs) { a[i] = (float)x[ia[i]]; b[i] = (float)x[ib[i]]; }
-            sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = 2 * p.pairs + lane + 64 * i;
-            u[i] = d < p.D ? (float)x[d] : 0.0f;
-            sum = fmaf(u[i], u[i], sum);
-        }
-        float f = 1.0f;
+        float a[N], b[N];
+        floats_of<T, N>(ra, a);
+        floats_of<T, N>(rb, b);
+        if (row + RPB < nt * H) fetch(row + RPB);
         if (p.norm != BX_NORM_NONE) {
-            sum = bx_wave_sum(sum);
-            f = p.norm == BX_NORM_RMS ? 1.0f / sqrtf(sum / (float)p.D + p.eps) : 1.0f / (sqrtf(sum) < p.eps ? p.eps : sqrtf(sum));
-        }
+            float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int pr = lane + 64 * i;
-            if (pr >= p.pairs) continue;
-            const float av = a[i] * f * (w ? (float)w[ia[i]] : 1.0f), bv = b[i] * f * (w ? (float)w[ib[i]] : 1.0f);
-            const float c = sc[pr], s = ss[pr];
-            y[ia[i]] = (T)(av * c - bv * s);
-            y[ib[i]] = (T)(bv * c + av * s);
-        }
+            for (int i = 0; i < N; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = 2 * p.pairs + lane + 64 * i;
-            if (d < p.D) y[d] = (T)(u[i] * f * (w ? (float)w[d] : 1.0f));
+            for (int k = LPR / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, LPR);
+            const float l2 = sqrtf(sum);
+            const float f = p.norm == BX_NORM_RMS ? 1.0f / sqrtf(sum / (float)p.D + p.eps) : 1.0f / (l2 < p.eps ? p.eps : l2);
+#pragma unroll
+            for (int i = 0; i < N; ++i) { a[i] *= f; b[i] *= f; }
         }
+        if (w) {
+            float wa[N], wb[N];
+            floats_of<T, N>(load_piece<T, N, VEC>(w + e0, n0), wa);
+            floats_of<T, N>(load_piece<T, N, VEC>(w + e1, n1), wb);
+#pragma unroll
+            for (int i = 0; i < N; ++i) { a[i] *= wa[i]; b[i] *= wb[i]; }
+        }
+        if (turn) {
+            const float *c = cs + t * P + N * x, *s = sn + t * P + N * x;
+            if constexpr (HALF) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float ci = VEC || i < n0 ? c[i] : 0.0f, si = VEC || i < n0 ? s[i] : 0.0f, v = a[i];
+                    a[i] = v * ci - b[i] * si;
+                    b[i] = b[i] * ci + v * si;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    float& v0 = i < N / 2 ? a[2 * i] : b[2 * i - N];
+                    float& v1 = i < N / 2 ? a[2 * i + 1] : b[2 * i + 1 - N];
+                    const bool is = VEC || N * x + i < P;
+                    const float ci = is ? c[i] : 0.0f, si = is ? s[i] : 0.0f, v = v0;
+                    v0 = v * ci - v1 * si;
+                    v1 = v1 * ci + v * si;
+                }
+            }
+        }
+        store_piece<T, N, VEC>(out + e0, a, n0);
+        store_piece<T, N, VEC>(out + e1, b, n1);
+    }
+}
+
+template <class T, int LPR, int N>
+int rope_launch(hipStream_t s, const RopeK& k, bool vec, int tpb, unsigned grid)
+{
+    const size_t lds = (size_t)tpb * k.pairs * 8;
+    if (k.half) {
+        if (vec) rope_kernel<T, LPR, N, true, true><<<grid, 256, lds, s>>>(k, tpb);
+        else rope_kernel<T, LPR, N, true, false><<<grid, 256, lds, s>>>(k, tpb);
+    } else {
+        if (vec) rope_kernel<T, LPR, N, false, true><<<grid, 256, lds, s>>>(k, tpb);
+        else rope_kernel<T, LPR, N, false, false><<<grid, 256, lds, s>>>(k, tpb);
+    }
+    BX_LAUNCH_CHECK();
+    return BX_OK;
+}
+
+template <class T>
+int rope_of(hipStream_t s, int n_cu, const RopeK& k)
+{
+    constexpr int N = BxElem<T>::CH;
+    const auto al = [](const void* p, long long x, long long y) { return (((uintptr_t)p | (uintptr_t)(x * (long long)sizeof(T)) | (uintptr_t)(y * (long long)sizeof(T))) & 15) == 0; };
+    const bool vec = k.pairs % N == 0 && (k.D - 2 * k.pairs) % (2 * N) == 0 && (k.Hq == 0 || (al(k.q, k.qs_t, k.qs_h) && al(k.qo, k.qos_t, k.qos_h) && al(k.qw, 0, 0))) &&
+                     (k.Hk == 0 || (al(k.k, k.ks_t, k.ks_h) && al(k.ko, k.kos_t, k.kos_h) && al(k.kw, 0, 0)));
+    // lanes of a row: its pairs N a lane, then what is not rotated 2 N a lane
+    const int lanes = (k.pairs + N - 1) / N + (k.D - 2 * k.pairs + 2 * N - 1) / (2 * N);
+    const int lpr = lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
+    // Tokens of a workgroup: about four head rows per lane group, so that the angles' latency is paid once for several rows and
+    // neighbouring rows are in flight together; fewer when the tokens would not fill the card, and no more than 48 KB of angles.
+    const int H = k.Hq + k.Hk, rpb = 256 / lpr;
+    long long tpb = (4LL * rpb + H - 1) / H;
+    const long long fill = (k.T + 4LL * n_cu - 1) / (4LL * n_cu);
+    if (tpb > fill) tpb = fill;
+    if (k.pairs > 0 && tpb > 49152 / (8 * k.pairs)) tpb = 49152 / (8 * k.pairs);
+    if (tpb < 1) tpb = 1;
+    const unsigned grid = (unsigned)((k.T + tpb - 1) / tpb);
+    switch (lpr) {
+        case 1: return rope_launch<T, 1, N>(s, k, vec, (int)tpb, grid);
+        case 2: return rope_launch<T, 2, N>(s, k, vec, (int)tpb, grid);
+        case 4: return rope_launch<T, 4, N>(s, k, vec, (int)tpb, grid);
+        case 8: return rope_launch<T, 8, N>(s, k, vec, (int)tpb, grid);
+        case 16: return rope_launch<T, 16, N>(s, k, vec, (int)tpb, grid);
+        case 32: return rope_launch<T, 32, N>(s, k, vec, (int)tpb, grid);
+        default: return rope_launch<T, 64, N>(s, k, vec, (int)tpb, grid);
     }
 }
 
@@ -110,16 +229,13 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeK p)
 
 int bxk_qk_norm_rope(hipStream_t s, int n_cu, const bx_qk_norm_rope_args& a)
 {
-    (void)n_cu;
     RopeK k = {a.q, a.k, a.pos, a.q_weight, a.k_weight, a.q_out, a.k_out, a.freqs, a.m_dev,
                a.q_stride_t, a.q_stride_h, a.k_stride_t, a.k_stride_h, a.q_out_stride_t, a.q_out_stride_h, a.k_out_stride_t, a.k_out_stride_h,
                a.pos_stride_t, (int)a.T, a.q ? a.Hq : 0, a.k ? a.Hk : 0, a.D, 0, a.axes, {0, 0, 0, 0}, a.norm, a.pairs == BX_PAIRS_HALF,
                a.pos_dtype == BX_POS_I32, a.eps};
     for (int i = 0; i < a.axes; ++i) { k.sec[i] = a.sections[i]; k.pairs += a.sections[i]; }
     if (k.T == 0 || k.Hq + k.Hk == 0) return BX_OK;
-    if (a.dtype == BX_TYPE_F32) rope_kernel<float><<<k.T, 256, 0, s>>>(k);
-    else if (a.dtype == BX_TYPE_F16) rope_kernel<bx_f16><<<k.T, 256, 0, s>>>(k);
-    else rope_kernel<bx_bf16><<<k.T, 256, 0, s>>>(k);
-    BX_LAUNCH_CHECK();
-    return BX_OK;
+    if (a.dtype == BX_TYPE_F32) return rope_of<float>(s, n_cu, k);
+    if (a.dtype == BX_TYPE_F16) return rope_of<bx_f16>(s, n_cu, k);
+    return rope_of<bx_bf16>(s, n_cu, k);
 }
