@@ -5,13 +5,31 @@
 
 namespace {
 
-__device__ __forceinline__ float act_of(float v, int act)
+// Both activations go by |v| and the power 2^(-..) of it, so nothing overflows and small results keep their relative precision.
+//   silu: v s (v >= 0) or v e s (v < 0),  e = exp(-|v|), s = 1 / (1 + e)
+//   gelu: v (1 - q) or v q,  q = Phi(-|v|) = exp(-v^2 / 2) t h(t),  t = 1 / (1 + 0.2625 |v|): h by the polynomial of degree 8 that fits
+//         0.5 erfcx(|v| / sqrt 2) / t with the least relative error (2e-8 over 0 .. 14.5).  20 instruction slots, where erfc takes over 50:
+//         at 67 million outputs that is a third of the time of the product itself.
+template <int act> __device__ __forceinline__ float act_of(float v)
 {
+    if (act == BX_ACT_NONE) return v;
     if (act == BX_ACT_RELU) return v > 0.0f ? v : (v != v ? v : 0.0f);
-    // erfc keeps the relative precision that 1 + erf loses for negative arguments
-    if (act == BX_ACT_GELU) return 0.5f * v * erfcf(-v * 0.70710678118654752f);
-    if (act == BX_ACT_SILU) return v / (1.0f + expf(-v));
-    return v;
+    if (act == BX_ACT_SILU) {
+        const float e = __builtin_amdgcn_exp2f(fabsf(v) * -1.44269504f), s = __builtin_amdgcn_rcpf(1.0f + e);
+        return v * (v >= 0.0f ? s : e * s);
+    }
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.2625f, fabsf(v), 1.0f));
+    float h = 0.0305265988f;
+    h = fmaf(h, t, -0.147754029f);
+    h = fmaf(h, t, 0.232594151f);
+    h = fmaf(h, t, -0.130927997f);
+    h = fmaf(h, t, 0.147445404f);
+    h = fmaf(h, t, 0.056567913f);
+    h = fmaf(h, t, 0.102634909f);
+    h = fmaf(h, t, 0.104164678f);
+    h = fmaf(h, t, 0.104748362f);
+    const float q = h * t * __builtin_amdgcn_exp2f(v * v * -0.72134752f);
+    return v * (v >= 0.0f ? 1.0f - q : q);
 }
 
 struct LinearK {
@@ -19,7 +37,7 @@ struct LinearK {
     void* y;
     const int32_t* m_dev;
     long long ldx, ldw, ldr, ldy;
-    int M, N, K, act, tiles_n;
+    int M, N, K, act, tiles_n, tiles_m;
 };
 
 template <class T>
@@ -29,7 +47,10 @@ __device__ __forceinline__ void epilogue4(const LinearK& p, int m, int n, const 
     float v[4], b[4] = {0.f, 0.f, 0.f, 0.f};
     if (p.bias) bx_load4<T>((const T*)p.bias + n, b, left);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = act_of(acc[j] + b[j], p.act);
+    for (int j = 0; j < 4; ++j) {
+        const float x = acc[j] + b[j];
+        v[j] = p.act == BX_ACT_RELU ? act_of<BX_ACT_RELU>(x) : p.act == BX_ACT_GELU ? act_of<BX_ACT_GELU>(x) : p.act == BX_ACT_SILU ? act_of<BX_ACT_SILU>(x) : x;
+    }
     if (p.residual) {
         float r[4];
         bx_load4<T>((const T*)p.residual + (long long)m * p.ldr + n, r, left);
@@ -39,45 +60,110 @@ __device__ __forceinline__ void epilogue4(const LinearK& p, int m, int n, const 
     bx_store4<T>((T*)p.y + (long long)m * p.ldy + n, v, left);
 }
 
+// CH consecutive columns (16 bytes) of one row of y, of which `left` exist
+template <class T> __device__ __forceinline__ void load_piece(const T* __restrict__ p, float* v, int left)
+{
+    constexpr int CH = BxElem<T>::CH;
+    T e[CH];
+    if (left >= CH) { const bxi4 r = reinterpret_cast<const BxAny16*>(p)->v; __builtin_memcpy(e, &r, 16); }
+    else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) e[j] = j < left ? p[j] : (T)0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < CH; ++j) v[j] = (float)e[j];
+}
+template <class T, int ACT> __device__ __forceinline__ void finish_piece(const LinearK& p, int m, int n, float* v, const float* bias)
+{
+    constexpr int CH = BxElem<T>::CH;
+    const int left = p.N - n;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) v[j] = act_of<ACT>(v[j] + bias[j]);
+    if (p.residual) {
+        float r[CH];
+        load_piece<T>((const T*)p.residual + (long long)m * p.ldr + n, r, left);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) v[j] += r[j];
+    }
+    T e[CH];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) e[j] = (T)v[j];
+    T* y = (T*)p.y + (long long)m * p.ldy + n;
+    if (left >= CH) { bxi4 r; __builtin_memcpy(&r, e, 16); reinterpret_cast<BxAny16*>(y)->v = r; }
+    else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+            if (j < left) y[j] = e[j];
+    }
+}
+
+// A wave's part of y, from its accumulators (a lane holds 4 columns of a row here and there) to memory: 32 rows at a time are turned over in
+// the wave's own piece of LDS, so that whole lanes in a row write 32 TN neighbouring columns.  Without it a store wrote 16 bytes
+// of 32 rows each, and 16384 x 4096 bf16 outputs alone took 145 of the layer's 200 us.
+template <class T, int TM, int TN, int ACT>
+__device__ __forceinline__ void put_rows(const LinearK& p, bxf16 (&acc)[TN][TM], float* lds, int lane, int m0, int n0, int M)
+{
+    constexpr int CH = BxElem<T>::CH, W = TN * 32, LD = W + 4, LPR = W / CH, RPI = 64 / LPR;      // lanes of a row, rows of a pass
+    const int lr = lane & 31, h = lane >> 5, c = lane % LPR * CH, n = n0 + c;
+    float bias[CH];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) bias[j] = 0.0f;
+    if (p.bias && n < p.N) load_piece<T>((const T*)p.bias + n, bias, p.N - n);
+#pragma unroll
+    for (int b = 0; b < TM; ++b) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int a = 0; a < TN; ++a)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *(bxf4*)&lds[lr * LD + a * 32 + 8 * g + 4 * h] = (bxf4){acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+            const int r = i * RPI + lane / LPR, m = m0 + b * 32 + r;
+            float v[CH];
+#pragma unroll
+            for (int j = 0; j < CH; j += 4) {
+                const bxf4 f = *(const bxf4*)&lds[r * LD + c + j];
+                v[j] = f[0]; v[j + 1] = f[1]; v[j + 2] = f[2]; v[j + 3] = f[3];
+            }
+            if (m < M && n < p.N) finish_piece<T, ACT>(p, m, n, v, bias);
+        }
+    }
+}
+
 // One workgroup = a BM x BN tile of y; a wave holds a (BM / WGM) x (BN / WGN) part of it in 32 x 32 accumulators.  The matrix product is
 // taken transposed (W rows as the first operand): a lane then holds four consecutive columns of one row of y and stores them together.
-// A row slice of 128 bytes is 8 chunks in LDS; chunk c of row r sits at c ^ (r & 7), so that the 8 lanes of a 128-byte LDS access
-// (consecutive rows, same chunk) meet 8 different bank groups.
-template <class T, int BM, int BN, int WGM, int WGN, bool ALIGNED>
-__global__ __launch_bounds__(WGM * WGN * 64) void linear_tile_kernel(LinearK p)
+// A row slice of 128 bytes is 8 chunks in LDS; chunk c of row r sits at c ^ (r / 2 % 8), so that the 16 lanes that one cycle of LDS serves
+// (consecutive rows, same chunk) meet all 64 banks.
+//
+// DIRECT: rows that are 16-byte aligned go from memory straight into LDS, one slice ahead of the products; what K leaves behind the last
+// whole slice, and rows that are not aligned, go through registers, where the elements behind K become zeros.  Rows behind the
+// last one repeat it: their products are not stored.
+//
+// KS > 1: so many groups of waves take the slices of K in turn, each with its own buffers, and meet in LDS at the end -- for outputs that are
+// too few to fill the card with tiles, where a workgroup's time is that of its loads one after the other.
+template <class T, int BM, int BN, int WGM, int WGN, int KS, bool DIRECT>
+__global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(LinearK p)
 {
-    constexpr int CH = BxElem<T>::CH, BK = 8 * CH, NT = WGM * WGN * 64;
+    constexpr int CH = BxElem<T>::CH, BK = 8 * CH, NW = WGM * WGN, NT = NW * 64;
     constexpr int TM = BM / WGM / 32, TN = BN / WGN / 32;
     constexpr int LX = BM * 8 / NT, LW = BN * 8 / NT;
-    __shared__ bxi4 sx[2][BM * 8], sw[2][BN * 8];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int m0 = (int)(blockIdx.x / p.tiles_n) * BM, n0 = (int)(blockIdx.x % p.tiles_n) * BN;
+    static_assert(NT % 128 == 0, "a thread's rows are a multiple of 16 apart: its chunks keep their place in a row");
+    constexpr int PUT = NW * 32 * (TN * 32 + 4) / 4, SLICES = 2 * (BM + BN) * 8;
+    __shared__ bxi4 lds[PUT > KS * SLICES ? PUT : KS * SLICES];
+    const int group = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+    bxi4 *const sx0 = lds + group * SLICES, *const sw0 = sx0 + BM * 8, *const sx1 = sw0 + BN * 8, *const sw1 = sx1 + BM * 8;
+    const int tid = threadIdx.x % NT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // tiles in groups of 8 rows of tiles, down the rows first: the tiles that an XCD works on at a time share rows of x and of W
+    const int id = (int)bx_xcd_order<32>(blockIdx.x, gridDim.x), gsize = 8 * p.tiles_n, first = id / gsize * 8, gm = min(8, p.tiles_m - first);
+    const int m0 = (first + id % gsize % gm) * BM, n0 = (id % gsize / gm) * BN;
     int M = p.M;
     if (p.m_dev) { const int live = *p.m_dev; M = live < M ? live : M; }
     if (m0 >= M) return;
-    const T* x = (const T*)p.x;
-    const T* w = (const T*)p.w;
-    bxi4 rx[LX], rw[LW];
-    const bxi4 zero = {0, 0, 0, 0};
-
-    auto fetch = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < LX; ++i) {
-            const int id = tid + i * NT, r = id >> 3, c = id & 7;
-            rx[i] = m0 + r < M ? bx_load_chunk<T, ALIGNED>(x + (long long)(m0 + r) * p.ldx, k0 + c * CH, p.K) : zero;
-        }
-#pragma unroll
-        for (int i = 0; i < LW; ++i) {
-            const int id = tid + i * NT, r = id >> 3, c = id & 7;
-            rw[i] = n0 + r < p.N ? bx_load_chunk<T, ALIGNED>(w + (long long)(n0 + r) * p.ldw, k0 + c * CH, p.K) : zero;
-        }
-    };
-    auto stage = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < LX; ++i) { const int id = tid + i * NT, r = id >> 3; sx[buf][r * 8 + ((id & 7) ^ (r & 7))] = rx[i]; }
-#pragma unroll
-        for (int i = 0; i < LW; ++i) { const int id = tid + i * NT, r = id >> 3; sw[buf][r * 8 + ((id & 7) ^ (r & 7))] = rw[i]; }
-    };
+    const T* x = (const T*)p.x + (long long)m0 * p.ldx;
+    const T* w = (const T*)p.w + (long long)n0 * p.ldw;
+    const int last_m = M - 1 - m0, last_n = p.N - 1 - n0;
 
     bxf16 acc[TN][TM];
 #pragma unroll
@@ -88,41 +174,119 @@ __global__ __launch_bounds__(WGM * WGN * 64) void linear_tile_kernel(LinearK p)
             for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.0f;
 
     const int wm = (wave / WGN) * TM * 32, wn = (wave % WGN) * TN * 32, lr = lane & 31, h = lane >> 5;
-    const int steps = (p.K + BK - 1) / BK;
-    if (steps > 0) { fetch(0); stage(0); }
-    for (int s = 0; s < steps; ++s) {
-        __syncthreads();
-        if (s + 1 < steps) fetch((s + 1) * BK);
-        const bxi4 *bx = sx[s & 1], *bw = sw[s & 1];
+    // LDS addresses: the swizzle is an XOR of address bits below a row
+    const int x_at = (wm + lr) * 128 + ((h ^ (lr >> 1 & 7)) * 16), w_at = (wn + lr) * 128 + ((h ^ (lr >> 1 & 7)) * 16);
+    const auto multiply = [&](const bxi4* sx, const bxi4* sw) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             bxi4 fx[TM], fw[TN];
 #pragma unroll
-            for (int b = 0; b < TM; ++b) { const int r = wm + b * 32 + lr; fx[b] = bx[r * 8 + ((2 * c + h) ^ (r & 7))]; }
+            for (int b = 0; b < TM; ++b) fx[b] = *(const bxi4*)((const char*)sx + (x_at ^ (c * 32)) + b * 32 * 128);
 #pragma unroll
-            for (int a = 0; a < TN; ++a) { const int r = wn + a * 32 + lr; fw[a] = bw[r * 8 + ((2 * c + h) ^ (r & 7))]; }
+            for (int a = 0; a < TN; ++a) fw[a] = *(const bxi4*)((const char*)sw + (w_at ^ (c * 32)) + a * 32 * 128);
 #pragma unroll
             for (int a = 0; a < TN; ++a)
 #pragma unroll
                 for (int b = 0; b < TM; ++b) acc[a][b] = bx_mma32<T>(fw[a], fx[b], acc[a][b]);
         }
-        if (s + 1 < steps) stage((s + 1) & 1);
+    };
+
+    // a slice through registers
+    bxi4 rx[LX], rw[LW];
+    const auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            const int e = tid + i * NT;
+            rx[i] = bx_load_chunk<T, DIRECT>(x + (long long)min(e >> 3, last_m) * p.ldx, k0 + (e & 7) * CH, p.K);
+        }
+#pragma unroll
+        for (int i = 0; i < LW; ++i) {
+            const int e = tid + i * NT;
+            rw[i] = bx_load_chunk<T, DIRECT>(w + (long long)min(e >> 3, last_n) * p.ldw, k0 + (e & 7) * CH, p.K);
+        }
+    };
+    const auto stage = [&](bxi4* sx, bxi4* sw) {
+#pragma unroll
+        for (int i = 0; i < LX; ++i) { const int e = tid + i * NT, r = e >> 3; sx[r * 8 + ((e & 7) ^ (r >> 1 & 7))] = rx[i]; }
+#pragma unroll
+        for (int i = 0; i < LW; ++i) { const int e = tid + i * NT, r = e >> 3; sw[r * 8 + ((e & 7) ^ (r >> 1 & 7))] = rw[i]; }
+    };
+
+    if constexpr (DIRECT) {
+        const int whole = p.K / BK;
+        const int c0 = ((tid & 7) ^ (tid >> 4 & 7)) * 16;
+        unsigned xo[LX], wo[LW];                             // the host sees to it that a tile's rows lie within 32 bits
+#pragma unroll
+        for (int i = 0; i < LX; ++i) xo[i] = (unsigned)min((tid + i * NT) >> 3, last_m) * (unsigned)(p.ldx * sizeof(T)) + c0;
+#pragma unroll
+        for (int i = 0; i < LW; ++i) wo[i] = (unsigned)min((tid + i * NT) >> 3, last_n) * (unsigned)(p.ldw * sizeof(T)) + c0;
+        const auto load = [&](bxi4* sx, bxi4* sw, int s) __attribute__((always_inline)) {
+            const char *xs = (const char*)x + (long long)s * 128, *ws = (const char*)w + (long long)s * 128;
+#pragma unroll
+            for (int i = 0; i < LX; ++i) bx_load_lds16(xs + xo[i], sx + i * NT + wave * 64);
+#pragma unroll
+            for (int i = 0; i < LW; ++i) bx_load_lds16(ws + wo[i], sw + i * NT + wave * 64);
+        };
+        if (group < whole) load(sx0, sw0, group);
+        for (int s = group, i = 0; i < (whole + KS - 1) / KS; s += KS, ++i) {
+            __syncthreads();
+            const bool odd = i & 1;
+            if (s + KS < whole) load(odd ? sx0 : sx1, odd ? sw0 : sw1, s + KS);
+            if (KS == 1 || s < whole) multiply(odd ? sx1 : sx0, odd ? sw1 : sw0);
+        }
+        if (whole * BK < p.K) {
+            if (group == 0) fetch(whole * BK);
+            __syncthreads();
+            if (group == 0) stage(sx0, sw0);
+            __syncthreads();
+            if (group == 0) multiply(sx0, sw0);
+        }
+    } else {
+        const int steps = (p.K + BK - 1) / BK;
+        if (group < steps) { fetch(group * BK); stage(sx0, sw0); }
+        for (int s = group, i = 0; i < (steps + KS - 1) / KS; s += KS, ++i) {
+            __syncthreads();
+            const bool odd = i & 1;
+            if (s + KS < steps) fetch((s + KS) * BK);
+            if (KS == 1 || s < steps) multiply(odd ? sx1 : sx0, odd ? sw1 : sw0);
+            if (s + KS < steps) stage(odd ? sx0 : sx1, odd ? sw0 : sw1);
+        }
+    }
+    if constexpr (KS > 1) {
+        // the groups' sums, added in their order
+        constexpr int A = TN * TM * 4;
+        static_assert((KS - 1) * NW * 64 * A <= KS * SLICES, "the groups' sums fit the buffers");
+        __syncthreads();
+        bxf4* sums = (bxf4*)lds;
+        if (group > 0) {
+#pragma unroll
+            for (int j = 0; j < A; ++j) {
+                const bxf16& f = acc[j / 4 / TM][j / 4 % TM];
+                sums[(((group - 1) * NW + wave) * A + j) * 64 + lane] = (bxf4){f[j % 4 * 4], f[j % 4 * 4 + 1], f[j % 4 * 4 + 2], f[j % 4 * 4 + 3]};
+            }
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll 1
+            for (int g = 0; g < KS - 1; ++g)
+#pragma unroll
+                for (int j = 0; j < A; ++j) {
+                    bxf16& f = acc[j / 4 / TM][j / 4 % TM];
+                    const bxf4 v = sums[((g * NW + wave) * A + j) * 64 + lane];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[j % 4 * 4 + i] += v[i];
+                }
+        }
+        __syncthreads();
+        if (group > 0) return;
     }
 
-#pragma unroll
-    for (int b = 0; b < TM; ++b) {
-        const int m = m0 + wm + b * 32 + lr;
-        if (m >= M) continue;
-#pragma unroll
-        for (int a = 0; a < TN; ++a)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int n = n0 + wn + a * 32 + 8 * g + 4 * h;
-                if (n >= p.N) continue;
-                const float v[4] = {acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
-                epilogue4<T>(p, m, n, v);
-            }
-    }
+    if (KS == 1) __syncthreads();
+    float* mine = (float*)lds + wave * 32 * (TN * 32 + 4);
+    if (p.act == BX_ACT_NONE) put_rows<T, TM, TN, BX_ACT_NONE>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
+    else if (p.act == BX_ACT_RELU) put_rows<T, TM, TN, BX_ACT_RELU>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
+    else if (p.act == BX_ACT_GELU) put_rows<T, TM, TN, BX_ACT_GELU>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
+    else put_rows<T, TM, TN, BX_ACT_SILU>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
 }
 
 // Few rows: one workgroup = 16 columns of y x 16 rows, its NW waves split K and meet in LDS.  Operands go from memory to the matrix
@@ -168,14 +332,16 @@ __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(LinearK p)
     }
 }
 
-template <class T, int BM, int BN, int WGM, int WGN>
+template <class T, int BM, int BN, int WGM, int WGN, int KS = 1>
 int launch_tile(hipStream_t s, LinearK k, bool aligned)
 {
     k.tiles_n = (k.N + BN - 1) / BN;
-    const long long tiles = (long long)k.tiles_n * ((k.M + BM - 1) / BM);
-    if (tiles > 0x7fffffffLL) { bx_set_error("bx_linear: %lld tiles exceed one launch", tiles); return BX_ERR_ARG; }
-    if (aligned) linear_tile_kernel<T, BM, BN, WGM, WGN, true><<<(unsigned)tiles, WGM * WGN * 64, 0, s>>>(k);
-    else linear_tile_kernel<T, BM, BN, WGM, WGN, false><<<(unsigned)tiles, WGM * WGN * 64, 0, s>>>(k);
+    k.tiles_m = (k.M + BM - 1) / BM;
+    const long long tiles = (long long)k.tiles_n * k.tiles_m;
+    if (tiles > 0x7fffffffLL || k.tiles_n > (1 << 27)) { bx_set_error("bx_linear: %lld tiles exceed one launch", tiles); return BX_ERR_ARG; }
+    const long long far = (1LL << 31) / (256 * (long long)sizeof(T));
+    if (aligned && k.ldx < far && k.ldw < far) linear_tile_kernel<T, BM, BN, WGM, WGN, KS, true><<<(unsigned)tiles, KS * WGM * WGN * 64, 0, s>>>(k);
+    else linear_tile_kernel<T, BM, BN, WGM, WGN, KS, false><<<(unsigned)tiles, KS * WGM * WGN * 64, 0, s>>>(k);
     BX_LAUNCH_CHECK();
     return BX_OK;
 }
@@ -183,19 +349,33 @@ int launch_tile(hipStream_t s, LinearK k, bool aligned)
 template <class T>
 int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
 {
-    LinearK k = {a.x, a.w, a.bias, a.residual, a.y, a.m_dev, a.ldx, a.ldw, a.ldr, a.ldy, (int)a.M, (int)a.N, (int)a.K, a.act, 0};
+    LinearK k = {a.x, a.w, a.bias, a.residual, a.y, a.m_dev, a.ldx, a.ldw, a.ldr, a.ldy, (int)a.M, (int)a.N, (int)a.K, a.act, 0, 0};
     const auto al16 = [](const void* p, long long ld) { return ((uintptr_t)p & 15) == 0 && (ld * (long long)sizeof(T)) % 16 == 0; };
     const bool aligned = al16(a.x, a.ldx) && al16(a.w, a.ldw);
-    const long long tiles64 = (long long)((k.M + 63) / 64) * ((k.N + 63) / 64);
-    if (k.M <= 32 || (tiles64 < n_cu / 2 && k.K >= 256)) {
+    const auto tiles = [&](int bm, int bn) { return (long long)((k.M + bm - 1) / bm) * ((k.N + bn - 1) / bn); };
+    // Few rows, or an output that 16 x 16 pieces fill the card with once: these read W (or x) straight from memory.  1 x 1024 x 1024 bf16:
+    // 4.2 us, 6.3 by the tiles below; 1000 x 32 by K = 512 f32: 6.0, 10.2; where there are more pieces they read too much again: 100 x 4096
+    // by K = 2048 bf16 28 us, 9.0 by tiles.
+    const long long pieces = tiles(16, 16);
+    if (k.M <= 16 || pieces <= n_cu) {
+        if (pieces > 0x7fffffffLL) { bx_set_error("bx_linear: %lld pieces exceed one launch", pieces); return BX_ERR_ARG; }
         k.tiles_n = (k.N + 15) / 16;
-        const long long g = (long long)k.tiles_n * ((k.M + 15) / 16);
-        if (aligned) linear_rows_kernel<T, 8, true><<<(unsigned)g, 512, 0, s>>>(k);
-        else linear_rows_kernel<T, 8, false><<<(unsigned)g, 512, 0, s>>>(k);
+        if (aligned) linear_rows_kernel<T, 8, true><<<(unsigned)pieces, 512, 0, s>>>(k);
+        else linear_rows_kernel<T, 8, false><<<(unsigned)pieces, 512, 0, s>>>(k);
         BX_LAUNCH_CHECK();
         return BX_OK;
     }
-    if ((long long)((k.M + 127) / 128) * ((k.N + 127) / 128) >= 2 * n_cu) return launch_tile<T, 128, 128, 2, 2>(s, k, aligned);
+    // Tiles that do not fill the card once: smaller ones with the slices of K dealt to four or two groups of waves.  32 x 4096 by K = 2048
+    // bf16 8.6 us (11.6 whole), 100 x 4096 9.0 (18.5), 300 x 4096 16.4 (19.7); f32 300 x 1024 by 1024 16.7 (25.6).
+    if (k.K > 16 * BxElem<T>::CH) {
+        if (k.M <= 32 && tiles(32, 64) <= n_cu) return launch_tile<T, 32, 64, 1, 2, 4>(s, k, aligned);
+        if (tiles(64, 32) <= n_cu) return launch_tile<T, 64, 32, 2, 1, 4>(s, k, aligned);
+        if (tiles(64, 64) <= n_cu) return launch_tile<T, 64, 64, 2, 2, 2>(s, k, aligned);
+    }
+    // Large outputs: halves want 256 x 256 (16384 x 4096 by K = 1024 with gelu 174 us; 175 by 128 x 128, 192 by 64 x 128), f32, whose
+    // matrix rate is a sixteenth, the smaller tiles' occupancy (10000 x 1024 by 1024: 171 us by 64 x 128, 195 by 64 x 64, 242 by 256 x 256).
+    if (sizeof(T) == 2 && tiles(256, 256) >= 2 * n_cu) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
+    if (k.N > 64 && tiles(64, 128) >= 4 * n_cu && k.K >= 256) return launch_tile<T, 64, 128, 2, 2>(s, k, aligned);
     return launch_tile<T, 64, 64, 2, 2>(s, k, aligned);
 }
 

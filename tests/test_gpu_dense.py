@@ -115,6 +115,20 @@ def test_linear_big_tiles(ctx, dt):
     _linear_case(ctx, dt, 4096, 1024, 256, act="none", residual=False)
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("M,N,K", [(20, 2100, 300), (31, 1056, 1024), (100, 1100, 520), (129, 640, 136), (300, 2000, 264), (1100, 300, 1031)])
+def test_linear_few_tiles(ctx, dt, pad, M, N, K):
+    """outputs that do not fill the card: the slices of K are dealt to groups of waves"""
+    _linear_case(ctx, dt, M, N, K, act="silu", pads=(pad, pad, 0, 0))
+
+
+@pytest.mark.parametrize("dt,M,N,K", [("f32", 8200, 1100, 264), ("bf16", 8230, 1030, 256), ("bf16", 33000, 1100, 72), ("f16", 33000, 1027, 100)])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_linear_many_tiles(ctx, dt, M, N, K, act):
+    _linear_case(ctx, dt, M, N, K, act=act, residual=act == "none")
+
+
 def test_linear_zero_sizes(ctx):
     for M, N, K in ((0, 5, 3), (5, 0, 3), (0, 0, 0)):
         assert ctx.linear(torch.zeros(M, K, device=DEV), torch.zeros(N, K, device=DEV)).shape == (M, N)
