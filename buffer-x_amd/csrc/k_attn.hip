@@ -51,7 +51,14 @@ __device__ __forceinline__ Span span_of(const AttnK& p, int b, int r0, int rows)
     return s;
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// the value of the lane 32 away
+__device__ __forceinline__ float other_half(float v)
+{
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    const unsigned x = __builtin_bit_cast(unsigned, v);
+    const u2 r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
 
 // The state of a wave's 32 rows and what one tile of 64 keys in LDS does to it.  K rows lie at chunk c ^ kswz(key), V rows at
 // c ^ vswz(key): the lanes of one LDS access then meet different banks.
@@ -66,11 +73,13 @@ struct Rows {
     bxf16 o[ND];
     bxi4 fq[CPR / 2];
     float m, thr, mb, l;
-    bool spoilt;                                             // of the wave
+    bool edge;                                               // of the wave
     int lane, lr, h;
 
-    static __device__ __forceinline__ int kswz(int key) { return CPR >= 8 ? key & 7 : (key >> 1) & 3; }
-    static __device__ __forceinline__ int vswz(int key) { return sizeof(T) == 4 ? 0 : CPR >= 8 ? (key & 3) << 1 : ((key >> 1) & 1) << 1; }
+    // 16 keys of the same chunk (one cycle of a 16-byte access), and 4 keys of 64 bytes (one cycle of the transposing one), each cover
+    // the 64 banks
+    static __device__ __forceinline__ int kswz(int key) { return CPR == 4 ? key >> 2 & 3 : CPR == 8 ? key >> 1 & 7 : CPR == 16 ? key & 15 : key & 7; }
+    static __device__ __forceinline__ int vswz(int key) { return sizeof(T) == 4 || CPR == 4 ? 0 : CPR == 8 ? (key >> 1 & 1) << 2 : (key & 3) << 2; }
 
     __device__ __forceinline__ void init(int lane_)
     {
@@ -88,7 +97,7 @@ struct Rows {
         m = thr = -INFINITY;
         mb = -BIAS;
         l = 0.0f;
-        spoilt = false;
+        edge = false;
     }
 
     // LDS addresses, in bytes from the tile's start.  The swizzles are XORs of address bits below a row, so that the chunks of a row are a
@@ -97,7 +106,7 @@ struct Rows {
     int k_at, v_at;                                          // set by init
     __device__ __forceinline__ bxi4 kfrag(const bxi4* sk, int k2, int c) const
     {
-        constexpr int M = CPR >= 8 ? 3 : 1;
+        constexpr int M = CPR == 4 ? 1 : CPR == 16 ? 7 : 3;
         return *(const bxi4*)((const char*)sk + (k_at ^ ((c & M) * 32)) + (c & ~M) * 32 + k2 * 32 * ROW);
     }
     // V^T operand of 16 keys (halves), in the order of S^T's registers
@@ -107,7 +116,7 @@ struct Rows {
         bxi4 f;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const char* a = (const char*)sv + (v_at ^ ((t & 1) * 64)) + (t >> 1) * 128 + (16 * u + 8 * g) * ROW;
+            const char* a = (const char*)sv + (v_at ^ (t * 64)) + (16 * u + 8 * g) * ROW;
             const bxi2 y = __builtin_bit_cast(bxi2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)a));
             f[2 * g] = y[0]; f[2 * g + 1] = y[1];
         }
@@ -138,28 +147,35 @@ struct Rows {
         return acc;
     }
 
-    // one tile: `masked` says whether sees(k2, i) -- does this lane's row see the key of register i of block k2 -- has to be asked
-    template <class See> __device__ __forceinline__ void tile(const bxi4* sk, const bxi4* sv, float c, float slack, bool masked, const See& sees)
+    // S^T of a tile: key(k2, c) is the operand of K for chunk pair c of block k2
+    struct Scores { bxf16 s[2]; };
+    template <class Key> __device__ __forceinline__ void score(const Key& key, Scores& x) const
     {
-        bxf16 s[2];
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[k2][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) x.s[k2][i] = 0.0f;
 #pragma unroll
-            for (int c2 = 0; c2 < CPR / 2; ++c2) s[k2] = bx_mma32<T>(kfrag(sk, k2, c2), fq[c2], s[k2]);
+            for (int c2 = 0; c2 < CPR / 2; ++c2) x.s[k2] = bx_mma32<T>(key(k2, c2), fq[c2], x.s[k2]);
         }
-        if (masked) {
-#pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[k2][i] = sees(k2, i) ? s[k2][i] : -INFINITY;
-        }
-        float mx = s[0][0];
+    }
+    // a tile on the edge of the mask: sees(j) says whether this lane's row sees the key that is j behind the lane's first
+    template <class See> __device__ __forceinline__ void hide(Scores& x, const See& sees)
+    {
+        edge = true;
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[k2][i]);
+            for (int i = 0; i < 16; ++i) x.s[k2][i] = sees(32 * k2 + 8 * (i / 4) + i % 4) ? x.s[k2][i] : -INFINITY;
+    }
+    // the rows' reference values follow where the tile's scores are too far above them
+    __device__ __forceinline__ void settle(const Scores& x, float c, float slack)
+    {
+        float mx = x.s[0][0];
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x.s[k2][i]);
         mx = fmaxf(mx, other_half(mx));
         if (__any(mx > thr)) {
             const float mn = fmaxf(m, mx);
@@ -173,54 +189,54 @@ struct Rows {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[t][i] *= alpha;
         }
+    }
+    __device__ __forceinline__ void weights(Scores& x, float c, Weights& w)
+    {
         float sum = 0.0f;
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[k2][i] = __builtin_amdgcn_exp2f(fmaf(s[k2][i], c, -mb));
-                sum += s[k2][i];
+                x.s[k2][i] = __builtin_amdgcn_exp2f(fmaf(x.s[k2][i], c, -mb));
+                sum += x.s[k2][i];
             }
         l += sum;
-        Weights w;
-        if constexpr (sizeof(T) == 4) { w.s[0] = s[0]; w.s[1] = s[1]; }
+        if constexpr (sizeof(T) == 4) { w.s[0] = x.s[0]; w.s[1] = x.s[1]; }
         else {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 T e[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = (T)s[u / 2][8 * (u % 2) + j];
+                for (int j = 0; j < 8; ++j) e[j] = (T)x.s[u / 2][8 * (u % 2) + j];
                 __builtin_memcpy(&w.f[u], e, 16);
             }
         }
-        // f32 sums a tile by itself first: fewer roundings at the size of O.  So do tiles on a mask's edge, to see whether anything
-        // but numbers came out: 0 times an infinity or NaN of a key that a row does not see would be in it (exact_rows).
-        if (masked) {
+    }
+    __device__ __forceinline__ void add(const bxi4* sv, const Weights& w)
+    {
 #pragma unroll
-            for (int t = 0; t < ND; ++t) {
-                bxf16 a;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) a[i] = 0.0f;
-                a = weigh(sv, w, t, a);
-                float z = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) { z = fmaf(a[i], 0.0f, z); o[t][i] += a[i]; }
-                spoilt |= __any(z != z);
-            }
-        } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int t = 0; t < ND; ++t) {
+        for (int t = 0; t < ND; ++t) {
+            if constexpr (sizeof(T) == 4) {
+                // f32 sums a tile by itself first: fewer roundings at the size of O
                 bxf16 a;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) a[i] = 0.0f;
                 a = weigh(sv, w, t, a);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[t][i] += a[i];
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < ND; ++t) o[t] = weigh(sv, w, t, o[t]);
+            } else o[t] = weigh(sv, w, t, o[t]);
         }
+    }
+    // Whether a wave that met the edge of a mask has anything but numbers in O: 0 times an infinity or NaN of a key that a row does not see
+    // would be in it (exact_rows).
+    __device__ __forceinline__ bool spoilt() const
+    {
+        float z = 0.0f;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z = fmaf(o[t][i], 0.0f, z);
+        return edge && __any(z != z);
     }
 };
 
@@ -313,7 +329,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
     const auto hi_of = [&](int i) { return p.right < 0 ? sp.kl : min(sp.kl, i + sp.off + p.right + 1); };
     const auto lo_of = [&](int i) { return p.left < 0 ? 0 : i + sp.off - p.left; };
     const int hi = live ? hi_of(qi) : 0, lo = lo_of(qi);
-    const int w_hi0 = hi_of(wi0), w_hi1 = hi_of(wi1), w_lo0 = lo_of(wi0), w_lo1 = lo_of(wi1);
+    const int w_hi0 = wave_live ? hi_of(wi0) : 0, w_hi1 = hi_of(wi1), w_lo0 = lo_of(wi0), w_lo1 = lo_of(wi1);
     {
         const T* qr = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
 #pragma unroll
@@ -322,16 +338,13 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
     const float slack = 8.0f / p.c;
 
     const auto base_of = [&](int t) { return (t < sp.t_sink ? t : sp.t_lo + t - sp.t_sink) * BN; };
-    const auto serve = [&](const bxi4* sk, const bxi4* sv, int t) __attribute__((always_inline)) {
+    const auto hide = [&](typename R_::Scores& x, int t) __attribute__((always_inline)) {
         const int j0 = base_of(t);
-        if (!wave_live || j0 >= w_hi1 || (j0 + BN <= w_lo0 && j0 >= p.sinks)) return;
-        const bool masked = !(j0 + BN <= w_hi0 && (j0 >= w_lo1 || j0 + BN <= p.sinks));
+        if (j0 + BN <= w_hi0 && (j0 >= w_lo1 || j0 + BN <= p.sinks)) return;
         const int a_hi = hi - j0 - 4 * h, a_lo = lo - j0 - 4 * h, a_sink = p.sinks - j0 - 4 * h;
-        w.tile(sk, sv, p.c, slack, masked, [&](int k2, int i) {
-            const int j = 32 * k2 + 8 * (i / 4) + i % 4;
-            return j < a_hi && (j >= a_lo || j < a_sink);
-        });
+        w.hide(x, [&](int j) { return j < a_hi && (j >= a_lo || j < a_sink); });
     };
+    const auto unseen = [&](int t) { const int j0 = base_of(t); return !wave_live || j0 >= w_hi1 || (j0 + BN <= w_lo0 && j0 >= p.sinks); };
 
     if constexpr (DIRECT) {
         // LDS position e holds chunk (e % CPR) ^ swizzle of key e / CPR.  Keys behind the sequence repeat its last one: no row sees
@@ -344,35 +357,66 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
         // A thread's keys of a tile are STEP apart, so its chunks keep their place within a row; the tile's address is the same for
         // all lanes and a lane adds 32 bits to it (the host sees to it that 64 rows stay within those).
         constexpr int STEP = NT / CPR;
-        static_assert(STEP % 8 == 0, "the swizzle of a thread's chunks does not depend on the key's step");
+        static_assert(STEP % (CPR == 32 ? 8 : 16) == 0, "the swizzle of a thread's chunks does not depend on the key's step");
         const int key0 = tid / CPR, ck = ((tid % CPR) ^ R_::kswz(key0)) * CH, cv = ((tid % CPR) ^ R_::vswz(key0)) * CH;
         const int wk = p.D < DP ? p.D : DP;
         const unsigned ks = (unsigned)(p.k_st * sizeof(T)), vs = (unsigned)(p.v_st * sizeof(T));
         const unsigned ko = key0 * ks + ck * (unsigned)sizeof(T), vo = key0 * vs + cv * (unsigned)sizeof(T);
-        const auto load = [&](bxi4* sk, bxi4* sv, int t) __attribute__((always_inline)) {
+        const auto load = [&](const T* base, long long st, unsigned bytes, unsigned off, int c, bxi4* to, int t) __attribute__((always_inline)) {
             const int j0 = base_of(t);
-            const char* kt = (const char*)(kb + (long long)j0 * p.k_st);
-            const char* vt = (const char*)(vb + (long long)j0 * p.v_st);
+            const char* first = (const char*)(base + (long long)j0 * st);
             const bool whole = j0 + BN <= sp.kl;
+            if (c < wk) {
 #pragma unroll
-            for (int i = 0; i < LD; ++i) {
-                const int e0 = (i * NW + wave) * 64;
-                if (whole) {
-                    if (ck < wk) bx_load_lds16(kt + (unsigned)(i * STEP) * ks + ko, sk + e0);
-                    if (cv < wk) bx_load_lds16(vt + (unsigned)(i * STEP) * vs + vo, sv + e0);
-                } else {
+                for (int i = 0; i < LD; ++i) {
                     const unsigned key = min(key0 + i * STEP, sp.kl - 1 - j0);
-                    if (ck < wk) bx_load_lds16(kt + (key * ks + ck * (unsigned)sizeof(T)), sk + e0);
-                    if (cv < wk) bx_load_lds16(vt + (key * vs + cv * (unsigned)sizeof(T)), sv + e0);
+                    bx_load_lds16(first + (whole ? (unsigned)(i * STEP) * bytes + off : key * bytes + c * (unsigned)sizeof(T)), to + (i * NW + wave) * 64);
                 }
             }
         };
-        if (t0 < t1) load(sk0, sv0, t0);
-        for (int t = t0; t < t1; ++t) {
-            bxi4 *ck_ = (t - t0) & 1 ? sk1 : sk0, *cv_ = (t - t0) & 1 ? sv1 : sv0, *nk_ = (t - t0) & 1 ? sk0 : sk1, *nv_ = (t - t0) & 1 ? sv0 : sv1;
+        const auto load_k = [&](int t) __attribute__((always_inline)) { load(kb, p.k_st, ks, ko, ck, (t - t0) & 1 ? sk1 : sk0, t); };
+        const auto load_v = [&](int t) __attribute__((always_inline)) { load(vb, p.v_st, vs, vo, cv, (t - t0) & 1 ? sv1 : sv0, t); };
+        const auto score = [&](typename R_::Scores& x, int t) __attribute__((always_inline)) {
+            const bxi4* sk = (t - t0) & 1 ? sk1 : sk0;
+            w.score([&](int k2, int c) { return w.kfrag(sk, k2, c); }, x);
+        };
+        // One step: the weights of tile t (the vector unit) while the scores of tile t + 1 are multiplied (the matrix unit), then the sums
+        // of tile t.  K runs one tile ahead of V, and both are loaded one step before they are read.
+        const auto step = [&](typename R_::Scores& now, typename R_::Scores& next, int t) __attribute__((always_inline)) {
             __syncthreads();
-            if (t + 1 < t1) load(nk_, nv_, t + 1);
-            serve(ck_, cv_, t);
+            if (t + 2 < t1) load_k(t + 2);
+            load_v(t + 1);
+            typename R_::Weights u;
+            score(next, t + 1);
+            w.weights(now, p.c, u);
+            w.add((t - t0) & 1 ? sv1 : sv0, u);
+            hide(next, t + 1);
+            w.settle(next, p.c, slack);
+        };
+        const auto finish = [&](typename R_::Scores& now) __attribute__((always_inline)) {
+            __syncthreads();
+            typename R_::Weights u;
+            w.weights(now, p.c, u);
+            w.add((t1 - 1 - t0) & 1 ? sv1 : sv0, u);
+        };
+        if (t0 < t1) {
+            typename R_::Scores a, b2;
+            load_k(t0);
+            __syncthreads();
+            if (t0 + 1 < t1) load_k(t0 + 1);
+            load_v(t0);
+            score(a, t0);
+            hide(a, t0);
+            w.settle(a, p.c, slack);
+            int t = t0;
+            for (; t + 2 < t1; t += 2) {
+                step(a, b2, t);
+                step(b2, a, t + 1);
+            }
+            if (t + 1 < t1) {
+                step(a, b2, t);
+                finish(b2);
+            } else finish(a);
         }
     } else {
         bxi4 rk[LD], rv[LD];
@@ -400,12 +444,19 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
             }
             __syncthreads();
             if (t + 1 < t1) fetch(t + 1);
-            serve(sk0, sv0, t);
+            if (unseen(t)) continue;
+            typename R_::Scores x;
+            typename R_::Weights u;
+            w.score([&](int k2, int c) { return w.kfrag(sk0, k2, c); }, x);
+            hide(x, t);
+            w.settle(x, p.c, slack);
+            w.weights(x, p.c, u);
+            w.add(sv0, u);
         }
     }
 
     const long long rows = (long long)p.B * p.Hk * p.Lq * p.G, part = (long long)split * rows + (long long)(b * p.Hk + hk) * p.Lq * p.G;
-    if (w.spoilt) {
+    if (w.spoilt()) {
         exact_rows<T>(p, sp, kb, vb, b, hk, w0, lane, t0, t1, DP, part, rows);
         return;
     }
@@ -438,49 +489,192 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
         }
 }
 
-// joins the parts of a row: weights 2^((m_s - m) c), in the order of the splits.  DP / 4 lanes per row, four dimensions each.
+// Up to 32 rows (single tokens and their like): the waves of a workgroup take the key tiles in turn instead of the rows, each on its own -- K straight
+// into the registers of the matrix instruction, V into the wave's piece of LDS -- and meet at the end.  Bound by memory: every wave has its
+// 64 keys of K and V in flight at once.
 template <class T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
+{
+    constexpr int CH = BxElem<T>::CH, CPR = DP / CH, NW = 4, LD = BN * CPR / 64;
+    using R_ = Rows<T, DP>;
+    __shared__ bxi4 sv_all[NW][BN * CPR];
+    __shared__ float sm[NW][32], sl[NW][32];
+    static_assert(BN * CPR * 16 >= 32 * DP * 4, "a wave's V holds its O");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int id = blockIdx.x;
+    const int split = id % p.nsplit; id /= p.nsplit;
+    const int hk = id % p.Hk, b = id / p.Hk;
+    const Span sp = span_of(p, b, 0, 32);
+    if (sp.R <= 0) return;
+    const int per = (sp.t_all + p.nsplit - 1) / p.nsplit;
+    const int t0 = min(sp.t_all, split * per), t1 = min(sp.t_all, t0 + per);
+    const T* kb = (const T*)p.k + (long long)b * p.k_sb + (long long)hk * p.k_sh;
+    const T* vb = (const T*)p.v + (long long)b * p.v_sb + (long long)hk * p.v_sh;
+    bxi4* sv = sv_all[wave];
+
+    R_ w;
+    w.init(lane);
+    const int h = w.h, lr = w.lr, row = min(lr, sp.R - 1), qi = row / p.G, qg = row - qi * p.G;
+    const auto hi_of = [&](int i) { return p.right < 0 ? sp.kl : min(sp.kl, i + sp.off + p.right + 1); };
+    const auto lo_of = [&](int i) { return p.left < 0 ? 0 : i + sp.off - p.left; };
+    const int hi = lr < sp.R ? hi_of(qi) : 0, lo = lo_of(qi), i1 = (sp.R - 1) / p.G;
+    const int w_hi0 = hi_of(0), w_lo1 = lo_of(i1);
+    {
+        const T* qr = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
+#pragma unroll
+        for (int c = 0; c < CPR / 2; ++c) w.fq[c] = bx_load_chunk<T, false>(qr, (2 * c + h) * CH, p.D);
+    }
+    const float slack = 8.0f / p.c;
+    if (p.D < DP) {
+        const bxi4 zero = {0, 0, 0, 0};
+        for (int e = lane; e < BN * CPR; e += 64) sv[e] = zero;
+    }
+    for (int t = t0 + wave; t < t1; t += NW) {
+        const int j0 = (t < sp.t_sink ? t : sp.t_lo + t - sp.t_sink) * BN;
+        // keys behind the sequence repeat its last one: no row sees them
+        bxi4 fk[2][CPR / 2];
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+            const T* kr = kb + (long long)min(j0 + 32 * k2 + lr, sp.kl - 1) * p.k_st;
+#pragma unroll
+            for (int c = 0; c < CPR / 2; ++c) fk[k2][c] = bx_load_chunk<T, true>(kr, (2 * c + h) * CH, p.D);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the last tile's V has been read
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int e = i * 64 + lane, key = e / CPR, cv = ((e % CPR) ^ R_::vswz(key)) * CH;
+            const T* vr = vb + (long long)min(j0 + key, sp.kl - 1) * p.v_st + cv;
+            if (cv < p.D) bx_load_lds16(vr, sv + i * 64);
+        }
+        const bool masked = !(j0 + BN <= w_hi0 && (j0 >= w_lo1 || j0 + BN <= p.sinks)) || sp.R < 32;
+        const int a_hi = hi - j0 - 4 * h, a_lo = lo - j0 - 4 * h, a_sink = p.sinks - j0 - 4 * h;
+        typename R_::Scores x;
+        typename R_::Weights u;
+        w.score([&](int k2, int c) { return fk[k2][c]; }, x);
+        if (masked) w.hide(x, [&](int j) { return j < a_hi && (j >= a_lo || j < a_sink); });
+        w.settle(x, p.c, slack);
+        w.weights(x, p.c, u);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's V is there
+        w.add(sv, u);
+    }
+    const long long rows = (long long)p.B * p.Hk * p.Lq * p.G, part = (long long)split * rows + (long long)(b * p.Hk + hk) * p.Lq * p.G;
+    if (__syncthreads_or(w.spoilt())) {
+        if (wave == 0) exact_rows<T>(p, sp, kb, vb, b, hk, 0, lane, t0, t1, DP, part, rows);
+        return;
+    }
+    // every wave lays its rows down in its piece of LDS; then four dimensions of a row a thread, the waves in their order
+    float* so = (float*)sv;
+#pragma unroll
+    for (int t = 0; t < R_::ND; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *(bxf4*)&so[lr * DP + (32 * t + 8 * g + 4 * h ^ (lr & 7) * 4)] = (bxf4){w.o[t][4 * g], w.o[t][4 * g + 1], w.o[t][4 * g + 2], w.o[t][4 * g + 3]};
+    const float l = w.l + other_half(w.l);
+    if (h == 0) { sm[wave][lr] = w.m; sl[wave][lr] = l; }
+    __syncthreads();
+    for (int e = tid; e < sp.R * (DP / 4); e += 256) {
+        const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+        if (d >= p.D && p.nsplit == 1) continue;
+        const float m = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+        const float mc = m == -INFINITY ? 0.0f : m * p.c;
+        float l4 = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+            const float f = __builtin_amdgcn_exp2f(fmaf(sm[x][r], p.c, -mc));
+            const bxf4 o = *(const bxf4*)&((const float*)sv_all[x])[r * DP + (d ^ (r & 7) * 4)];
+            l4 = fmaf(f, sl[x][r], l4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = fmaf(f, o[j], v[j]);
+        }
+        if (p.nsplit > 1) {
+            *reinterpret_cast<bxf4*>(p.ws + (part + r) * DP + d) = (bxf4){v[0], v[1], v[2], v[3]};
+            float* ml = p.ws + (long long)p.nsplit * rows * DP + (part + r) * 2;
+            if (d == 0) { ml[0] = m; ml[1] = l4; }
+        } else {
+            const int oi = r / p.G, og = r - oi * p.G;
+            const float inv = hi_of(oi) <= 0 ? 0.0f : 1.0f / l4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] *= inv;
+            bx_store4<T>((T*)p.o + (long long)b * p.o_sb + (long long)oi * p.o_st + (long long)(hk * p.G + og) * p.o_sh + d, v, p.D - d);
+        }
+    }
+}
+
+// joins the parts of a row: weights 2^((m_s - m) c).  DP / 4 lanes have four dimensions each; SG groups of them share the splits of a row and add up
+// in their order, so that a single token's many parts are read together instead of one after the other.
+template <class T, int DP, int SG>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
 {
-    constexpr int LPR = DP / 4, RPB = 256 / LPR;
-    const long long rows = (long long)p.B * p.Hk * p.Lq * p.G, at = (long long)blockIdx.x * RPB + threadIdx.x / LPR;
-    if (at >= rows) return;
-    const int d = threadIdx.x % LPR * 4;
+    constexpr int LPR = DP / 4, RPB = 256 / LPR / SG;
+    __shared__ float sm[RPB][SG], sl[RPB][SG];
+    __shared__ bxf4 so[RPB][SG][LPR];
+    const long long rows = (long long)p.B * p.Hk * p.Lq * p.G;
+    const int x = threadIdx.x % LPR, g = threadIdx.x / LPR % SG, rb = threadIdx.x / LPR / SG, d = x * 4;
+    const long long at = (long long)blockIdx.x * RPB + rb;
     const int per = p.Lq * p.G, r = (int)(at % per), bh = (int)(at / per), b = bh / p.Hk, hk = bh - b * p.Hk;
     const int qi = r / p.G, qg = r - qi * p.G;
-    const int ql = p.q_lens ? max(0, min(p.Lq, p.q_lens[b])) : p.Lq, kl = p.k_lens ? max(0, min(p.Lk, p.k_lens[b])) : p.Lk;
-    if (qi >= ql || d >= p.D) return;
+    const bool there = at < rows;
+    const int ql = there && p.q_lens ? max(0, min(p.Lq, p.q_lens[b])) : p.Lq, kl = there && p.k_lens ? max(0, min(p.Lk, p.k_lens[b])) : p.Lk;
+    const bool live = there && qi < ql;
     const float* ml = p.ws + (long long)p.nsplit * rows * DP;
     float m = -INFINITY;
-    for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, ml[((long long)s * rows + at) * 2]);
-    const float mc = m == -INFINITY ? 0.0f : m * p.c;
-    float l = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(ml[((long long)s * rows + at) * 2], p.c, -mc));
-        l = fmaf(w, ml[((long long)s * rows + at) * 2 + 1], l);
-        const bxf4 o = *reinterpret_cast<const bxf4*>(p.ws + ((long long)s * rows + at) * DP + d);
+    if (live)
+        for (int s = g; s < p.nsplit; s += SG) m = fmaxf(m, ml[((long long)s * rows + at) * 2]);
+    if constexpr (SG > 1) {
+        if (x == 0) sm[rb][g] = m;
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = fmaf(w, o[j], v[j]);
+        for (int j = 0; j < SG; ++j) m = fmaxf(m, sm[rb][j]);
     }
+    const float mc = m == -INFINITY ? 0.0f : m * p.c;
+    float l = 0.0f;
+    bxf4 v = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+#pragma unroll 4
+        for (int s = g; s < p.nsplit; s += SG) {
+            const long long i = (long long)s * rows + at;
+            const float w = __builtin_amdgcn_exp2f(fmaf(ml[i * 2], p.c, -mc));
+            const bxf4 o = *reinterpret_cast<const bxf4*>(p.ws + i * DP + d);
+            l = fmaf(w, ml[i * 2 + 1], l);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = fmaf(w, o[j], v[j]);
+        }
+    }
+    if constexpr (SG > 1) {
+        so[rb][g][x] = v;
+        if (x == 0) sl[rb][g] = l;
+        __syncthreads();
+        if (g > 0) return;
+#pragma unroll
+        for (int j = 1; j < SG; ++j) { v += so[rb][j][x]; l += sl[rb][j]; }
+    }
+    if (!live || d >= p.D) return;
     const bool empty = p.right >= 0 && qi + kl - ql + p.right + 1 <= 0;
     const float inv = empty || kl <= 0 ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] *= inv;
-    T* po = (T*)p.o + (long long)b * p.o_sb + (long long)qi * p.o_st + (long long)(hk * p.G + qg) * p.o_sh;
-    bx_store4<T>(po + d, v, p.D - d);
+    const float y[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+    bx_store4<T>((T*)p.o + (long long)b * p.o_sb + (long long)qi * p.o_st + (long long)(hk * p.G + qg) * p.o_sh + d, y, p.D - d);
 }
 
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-struct Shape { int DP, tiles_r, nsplit; };
+struct Shape { int DP, tiles_r, nsplit; bool rows; };
 
-// Rows alone fill the card when there are two workgroups a compute unit; with fewer the keys are split, as long as a part keeps
-// four tiles of 64 keys (below that the joining costs more than it saves).
+// whether rows of 16-byte aligned whole chunks let K and V skip the registers
+bool direct_of(const bx_attention_args& a)
+{
+    const int e = a.dtype == BX_TYPE_F32 ? 4 : 2;
+    const auto al = [e](const void* p, long long x, long long y, long long z) { return (((uintptr_t)p | (uintptr_t)(x * e) | (uintptr_t)(y * e) | (uintptr_t)(z * e)) & 15) == 0; };
+    const long long far = (1LL << 31) / (BN * e);            // rows further apart: a tile does not fit 32-bit offsets
+    return a.D * e % 16 == 0 && a.k_stride_t < far && a.v_stride_t < far && al(a.q, a.q_stride_b, a.q_stride_t, a.q_stride_h) &&
+           al(a.k, a.k_stride_b, a.k_stride_t, a.k_stride_h) && al(a.v, a.v_stride_b, a.v_stride_t, a.v_stride_h);
+}
+
 Shape shape_of(int n_cu, const bx_attention_args& a)
 {
     Shape s;
     s.DP = padded(a.D);
     const long long R = (long long)a.Lq * (a.Hq / a.Hk);
+    s.rows = R <= 32 && direct_of(a);
     s.tiles_r = (int)((R + 127) / 128);
     const long long base = (long long)s.tiles_r * a.Hk * a.B;
     long long keys = a.Lk;
@@ -489,8 +683,10 @@ Shape shape_of(int n_cu, const bx_attention_args& a)
         keys = span < keys ? span : keys;
     }
     const long long tiles = (keys + BN - 1) / BN;
+    // Rows alone fill the card when there are two workgroups a compute unit; with fewer the keys are split, as long as a part keeps four
+    // tiles of 64 keys (one per wave, or enough that joining does not cost more than it saves).
     long long n = base > 0 ? 2LL * n_cu / base : 1;
-    if (n > tiles / 4) n = tiles / 4;
+    if (n > (tiles + 3) / 4) n = (tiles + 3) / 4;
     if (n > 128) n = 128;
     s.nsplit = n < 1 ? 1 : (int)n;
     return s;
@@ -502,15 +698,19 @@ int64_t bytes_of(const Shape& s, const bx_attention_args& a)
     return (int64_t)s.nsplit * a.B * a.Lq * a.Hq * (s.DP + 2) * 4;
 }
 
-template <class T, int DP, bool DIRECT>
-int launch(hipStream_t s, const AttnK& k)
+template <class T, int DP>
+int launch(hipStream_t s, const AttnK& k, bool rows_form, bool direct)
 {
-    const long long grid = (long long)k.tiles_r * k.Hk * k.B * k.nsplit;
-    attn_kernel<T, DP, 4, DIRECT><<<(unsigned)grid, 256, 0, s>>>(k);
+    const unsigned grid = (unsigned)((long long)k.tiles_r * k.Hk * k.B * k.nsplit);
+    if (rows_form) attn_rows_kernel<T, DP><<<grid, 256, 0, s>>>(k);
+    else if (direct) attn_kernel<T, DP, 4, true><<<grid, 256, 0, s>>>(k);
+    else attn_kernel<T, DP, 4, false><<<grid, 256, 0, s>>>(k);
     BX_LAUNCH_CHECK();
     if (k.nsplit > 1) {
-        const long long rows = (long long)k.B * k.Hk * k.Lq * k.G, per = 256 / (DP / 4);
-        attn_join_kernel<T, DP><<<(unsigned)((rows + per - 1) / per), 256, 0, s>>>(k);
+        constexpr int SG = 32 * 8 / (DP / 4) > 8 ? 8 : 32 * 8 / (DP / 4);
+        const long long rows = (long long)k.B * k.Hk * k.Lq * k.G, whole = 256 / (DP / 4), shared = whole / SG;
+        if (k.nsplit > 8) attn_join_kernel<T, DP, SG><<<(unsigned)((rows + shared - 1) / shared), 256, 0, s>>>(k);
+        else attn_join_kernel<T, DP, 1><<<(unsigned)((rows + whole - 1) / whole), 256, 0, s>>>(k);
         BX_LAUNCH_CHECK();
     }
     return BX_OK;
@@ -520,20 +720,15 @@ template <class T>
 int attention_of(hipStream_t s, int n_cu, const bx_attention_args& a)
 {
     const Shape sh = shape_of(n_cu, a);
-    AttnK k = {a.q, a.k, a.v, a.o, a.q_lens, a.k_lens, (float*)a.workspace,
-               a.q_stride_b, a.q_stride_t, a.q_stride_h, a.k_stride_b, a.k_stride_t, a.k_stride_h,
-               a.v_stride_b, a.v_stride_t, a.v_stride_h, a.o_stride_b, a.o_stride_t, a.o_stride_h,
-               a.B, a.Lq, a.Lk, a.Hk, a.Hq / a.Hk, a.D, a.left, a.right, a.sinks, sh.nsplit, sh.tiles_r,
-               (float)((double)a.scale * 1.4426950408889634)};
-    const auto al = [](const void* p, long long x, long long y, long long z) {
-        return (((uintptr_t)p | (uintptr_t)(x * (long long)sizeof(T)) | (uintptr_t)(y * (long long)sizeof(T)) | (uintptr_t)(z * (long long)sizeof(T))) & 15) == 0;
-    };
-    const long long far = (1LL << 31) / (BN * (long long)sizeof(T));          // rows further apart: a tile does not fit 32-bit offsets
-    const bool direct = a.D % BxElem<T>::CH == 0 && a.k_stride_t < far && a.v_stride_t < far && al(a.q, a.q_stride_b, a.q_stride_t, a.q_stride_h) && al(a.k, a.k_stride_b, a.k_stride_t, a.k_stride_h) &&
-                        al(a.v, a.v_stride_b, a.v_stride_t, a.v_stride_h);
-    if (sh.DP == 32) return direct ? launch<T, 32, true>(s, k) : launch<T, 32, false>(s, k);
-    if (sh.DP == 64) return direct ? launch<T, 64, true>(s, k) : launch<T, 64, false>(s, k);
-    return direct ? launch<T, 128, true>(s, k) : launch<T, 128, false>(s, k);
+    const AttnK k = {a.q, a.k, a.v, a.o, a.q_lens, a.k_lens, (float*)a.workspace,
+                     a.q_stride_b, a.q_stride_t, a.q_stride_h, a.k_stride_b, a.k_stride_t, a.k_stride_h,
+                     a.v_stride_b, a.v_stride_t, a.v_stride_h, a.o_stride_b, a.o_stride_t, a.o_stride_h,
+                     a.B, a.Lq, a.Lk, a.Hk, a.Hq / a.Hk, a.D, a.left, a.right, a.sinks, sh.nsplit, sh.tiles_r,
+                     (float)((double)a.scale * 1.4426950408889634)};
+    const bool direct = direct_of(a);
+    if (sh.DP == 32) return launch<T, 32>(s, k, sh.rows, direct);
+    if (sh.DP == 64) return launch<T, 64>(s, k, sh.rows, direct);
+    return launch<T, 128>(s, k, sh.rows, direct);
 }
 
 }  // namespace
