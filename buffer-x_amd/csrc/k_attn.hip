@@ -617,36 +617,39 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
     const int ql = there && p.q_lens ? max(0, min(p.Lq, p.q_lens[b])) : p.Lq, kl = there && p.k_lens ? max(0, min(p.Lk, p.k_lens[b])) : p.Lk;
     const bool live = there && qi < ql;
     const float* ml = p.ws + (long long)p.nsplit * rows * DP;
-    float m = -INFINITY;
-    if (live)
-        for (int s = g; s < p.nsplit; s += SG) m = fmaxf(m, ml[((long long)s * rows + at) * 2]);
-    if constexpr (SG > 1) {
-        if (x == 0) sm[rb][g] = m;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < SG; ++j) m = fmaxf(m, sm[rb][j]);
-    }
-    const float mc = m == -INFINITY ? 0.0f : m * p.c;
-    float l = 0.0f;
+    // one pass with a running maximum; four parts are on their way at a time
+    float m = -INFINITY, l = 0.0f;
     bxf4 v = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-#pragma unroll 4
-        for (int s = g; s < p.nsplit; s += SG) {
-            const long long i = (long long)s * rows + at;
-            const float w = __builtin_amdgcn_exp2f(fmaf(ml[i * 2], p.c, -mc));
-            const bxf4 o = *reinterpret_cast<const bxf4*>(p.ws + i * DP + d);
-            l = fmaf(w, ml[i * 2 + 1], l);
+    const auto take = [&](float ms, float ls, const bxf4& o) {
+        const float mn = fmaxf(m, ms), mc = mn == -INFINITY ? 0.0f : mn * p.c;
+        const float a = __builtin_amdgcn_exp2f(fmaf(m, p.c, -mc)), w = __builtin_amdgcn_exp2f(fmaf(ms, p.c, -mc));
+        m = mn;
+        l = fmaf(l, a, w * ls);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = fmaf(w, o[j], v[j]);
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(v[j], a, w * o[j]);
+    };
+    if (live) {
+        for (int s0 = g; s0 < p.nsplit; s0 += 4 * SG) {
+            float ms[4], ls[4];
+            bxf4 o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const long long i = (long long)min(s0 + j * SG, p.nsplit - 1) * rows + at;
+                ms[j] = ml[i * 2]; ls[j] = ml[i * 2 + 1];
+                o[j] = *reinterpret_cast<const bxf4*>(p.ws + i * DP + d);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (s0 + j * SG < p.nsplit) take(ms[j], ls[j], o[j]);
         }
     }
     if constexpr (SG > 1) {
         so[rb][g][x] = v;
-        if (x == 0) sl[rb][g] = l;
+        if (x == 0) { sm[rb][g] = m; sl[rb][g] = l; }
         __syncthreads();
         if (g > 0) return;
 #pragma unroll
-        for (int j = 1; j < SG; ++j) { v += so[rb][j][x]; l += sl[rb][j]; }
+        for (int j = 1; j < SG; ++j) take(sm[rb][j], sl[rb][j], so[rb][j][x]);
     }
     if (!live || d >= p.D) return;
     const bool empty = p.right >= 0 && qi + kl - ql + p.right + 1 <= 0;

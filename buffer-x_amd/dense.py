@@ -49,93 +49,82 @@ def _operand(torch, name, t, device, dtype, shape):
     return t.data_ptr()
 
 
+def _sized(torch, name, t, dims, what):
+    if not (isinstance(t, torch.Tensor) and t.dim() == dims):
+        raise ValueError(f"{name} has to be a tensor {what}")
+    return t.shape
+
+
 def linear_args(torch, device, x, weight, bias, act, residual, out, m_dev):
-    _need(isinstance(x, torch.Tensor) and x.dim() == 2, "x has to be a tensor [M, K]")
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight has to be a tensor [N, K]")
-    _need(act in ACTS, f"unknown activation {act!r} (known: {tuple(ACTS)})")
-    (M, K), N, dt = x.shape, weight.shape[0], x.dtype
-    a = lib.BxLinearArgs()
-    a.dtype, a.act, a.M, a.N, a.K = _type(torch, x), ACTS[act], M, N, K
-    a.x, a.ldx = _operand(torch, "x", x, device, dt, (M, K)), x.stride(0)
-    a.w, a.ldw = _operand(torch, "weight", weight, device, dt, (N, K)), weight.stride(0)
-    if bias is not None:
-        a.bias = _operand(torch, "bias", bias, device, dt, (N,))
-    if residual is not None:
-        a.residual, a.ldr = _operand(torch, "residual", residual, device, dt, (M, N)), residual.stride(0)
-    if m_dev is not None:
-        a.m_dev = _operand(torch, "m_dev", m_dev, device, torch.int32, (1,))
+    M, K = _sized(torch, "x", x, 2, "[M, K]")
+    N = _sized(torch, "weight", weight, 2, "[N, K]")[0]
+    dt, code = x.dtype, _type(torch, x)
+    if act not in ACTS:
+        raise ValueError(f"unknown activation {act!r} (known: {tuple(ACTS)})")
+    px, pw = _operand(torch, "x", x, device, dt, (M, K)), _operand(torch, "weight", weight, device, dt, (N, K))
+    pb = None if bias is None else _operand(torch, "bias", bias, device, dt, (N,))
+    pr, ldr = (None, 0) if residual is None else (_operand(torch, "residual", residual, device, dt, (M, N)), residual.stride(0))
+    pm = None if m_dev is None else _operand(torch, "m_dev", m_dev, device, torch.int32, (1,))
     if out is None:
         out = torch.empty((M, N), dtype=dt, device=device)
-    a.y, a.ldy = _operand(torch, "out", out, device, dt, (M, N)), out.stride(0)
-    return a, out
+        py, ldy = out.data_ptr(), N
+    else:
+        py, ldy = _operand(torch, "out", out, device, dt, (M, N)), out.stride(0)
+    return lib.BxLinearArgs(code, ACTS[act], M, N, K, x.stride(0), weight.stride(0), ldr, ldy, px, pw, pb, pr, py, pm), out
+
+
+def _heads(torch, name, t, weight, out, device, dt, T, D):
+    """(heads, address, token and head stride, weight's address, out, its address and strides) of q or k; absent: all zero"""
+    if t is None:
+        if out is not None or weight is not None:
+            raise ValueError(f"{name}_out and {name}_weight need {name}")
+        return 0, None, 0, 0, None, None, None, 0, 0
+    H = _sized(torch, name, t, 3, "[T, heads, D]")[1]
+    at = _operand(torch, name, t, device, dt, (T, H, D))
+    w = None if weight is None else _operand(torch, name + "_weight", weight, device, dt, (D,))
+    st, sh, _ = t.stride()
+    if out is None:
+        out = torch.empty((T, H, D), dtype=dt, device=device)
+        return H, at, st, sh, w, out, out.data_ptr(), H * D, D
+    ot, oh, _ = out.stride() if isinstance(out, torch.Tensor) and out.dim() == 3 else (0, 0, 0)
+    return H, at, st, sh, w, out, _operand(torch, name + "_out", out, device, dt, (T, H, D)), ot, oh
 
 
 def qk_norm_rope_args(torch, device, q, k, pos, freqs, sections, norm, eps, q_weight, k_weight, pairs, q_out, k_out, m_dev):
-    _need(norm in NORMS, f"unknown norm {norm!r} (known: {tuple(NORMS)})")
-    _need(pairs in PAIRS, f"unknown order of pairs {pairs!r} (known: {tuple(PAIRS)})")
-    sections = tuple(int(s) for s in sections)
-    _need(1 <= len(sections) <= 4 and min(sections) >= 0, "sections: the rotation pairs of 1 to 4 axes")
+    if norm not in NORMS:
+        raise ValueError(f"unknown norm {norm!r} (known: {tuple(NORMS)})")
+    if pairs not in PAIRS:
+        raise ValueError(f"unknown order of pairs {pairs!r} (known: {tuple(PAIRS)})")
+    axes = len(sections)
+    _need(1 <= axes <= 4 and min(sections) >= 0, "sections: the rotation pairs of 1 to 4 axes")
     first = q if q is not None else k
-    _need(isinstance(first, torch.Tensor) and first.dim() == 3, "q and / or k have to be tensors [T, heads, D]")
-    T, _, D = first.shape
-    dt = first.dtype
-    a = lib.BxQkNormRopeArgs()
-    a.dtype, a.norm, a.pairs, a.T, a.D, a.axes, a.eps = _type(torch, first), NORMS[norm], PAIRS[pairs], T, D, len(sections), eps
-    for i, s in enumerate(sections):
-        a.sections[i] = s
-    _need(isinstance(pos, torch.Tensor) and pos.dtype in (torch.float32, torch.int32), "pos has to be a float32 or int32 tensor [T, axes]")
-    a.pos_dtype = 0 if pos.dtype is torch.float32 else 1
-    a.pos, a.pos_stride_t = _operand(torch, "pos", pos, device, pos.dtype, (T, len(sections))), pos.stride(0)
-    a.freqs = _operand(torch, "freqs", freqs, device, torch.float64, (sum(sections),))
-    if q is not None:
-        _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q has to be a tensor [T, heads, D]")
-        shape = (T, q.shape[1], D)
-        a.Hq, a.q, a.q_stride_t, a.q_stride_h = shape[1], _operand(torch, "q", q, device, dt, shape), q.stride(0), q.stride(1)
-        if q_out is None:
-            q_out = torch.empty(shape, dtype=dt, device=device)
-        a.q_out, a.q_out_stride_t, a.q_out_stride_h = _operand(torch, "q_out", q_out, device, dt, shape), q_out.stride(0), q_out.stride(1)
-        if q_weight is not None:
-            a.q_weight = _operand(torch, "q_weight", q_weight, device, dt, (D,))
-    else:
-        _need(q_out is None and q_weight is None, "q_out and q_weight need q")
-    if k is not None:
-        _need(isinstance(k, torch.Tensor) and k.dim() == 3, "k has to be a tensor [T, heads, D]")
-        shape = (T, k.shape[1], D)
-        a.Hk, a.k, a.k_stride_t, a.k_stride_h = shape[1], _operand(torch, "k", k, device, dt, shape), k.stride(0), k.stride(1)
-        if k_out is None:
-            k_out = torch.empty(shape, dtype=dt, device=device)
-        a.k_out, a.k_out_stride_t, a.k_out_stride_h = _operand(torch, "k_out", k_out, device, dt, shape), k_out.stride(0), k_out.stride(1)
-        if k_weight is not None:
-            a.k_weight = _operand(torch, "k_weight", k_weight, device, dt, (D,))
-    else:
-        _need(k_out is None and k_weight is None, "k_out and k_weight need k")
-    if m_dev is not None:
-        a.m_dev = _operand(torch, "m_dev", m_dev, device, torch.int32, (1,))
-    return a, q_out, k_out
+    T, _, D = _sized(torch, "q (or k, where q is None)", first, 3, "[T, heads, D]")
+    dt, code = first.dtype, _type(torch, first)
+    is_i32 = isinstance(pos, torch.Tensor) and pos.dtype is torch.int32
+    pp = _operand(torch, "pos (float32 or int32)", pos, device, torch.int32 if is_i32 else torch.float32, (T, axes))
+    pf = _operand(torch, "freqs", freqs, device, torch.float64, (sum(sections),))
+    pm = None if m_dev is None else _operand(torch, "m_dev", m_dev, device, torch.int32, (1,))
+    Hq, aq, qt, qh, wq, q_out, oq, oqt, oqh = _heads(torch, "q", q, q_weight, q_out, device, dt, T, D)
+    Hk, ak, kt, kh, wk, k_out, ok, okt, okh = _heads(torch, "k", k, k_weight, k_out, device, dt, T, D)
+    return lib.BxQkNormRopeArgs(code, NORMS[norm], PAIRS[pairs], int(is_i32), T, Hq, Hk, D, axes, tuple(sections), eps, 0, qt, qh, kt, kh, oqt, oqh, okt,
+                                okh, pos.stride(0), aq, ak, wq, wk, pp, pf, oq, ok, pm), q_out, k_out
 
 
 def attention_args(torch, device, q, k, v, scale, window, sinks, q_lens, k_lens, out):
-    _need(isinstance(q, torch.Tensor) and q.dim() == 4, "q has to be a tensor [B, Lq, heads, D]")
-    _need(isinstance(k, torch.Tensor) and k.dim() == 4, "k has to be a tensor [B, Lk, heads, D]")
-    B, Lq, Hq, D = q.shape
-    Lk, Hk, dt = k.shape[1], k.shape[2], q.dtype
-    a = lib.BxAttentionArgs()
-    a.dtype, a.B, a.Lq, a.Lk, a.Hq, a.Hk, a.D = _type(torch, q), B, Lq, Lk, Hq, Hk, D
-    a.left, a.right = (max(-1, min(int(w), 2**31 - 1)) for w in window)
-    a.sinks = min(int(sinks), 2**31 - 1)
-    a.scale = D ** -0.5 if scale is None and D > 0 else float(scale or 0.0)
-    a.q = _operand(torch, "q", q, device, dt, (B, Lq, Hq, D))
-    a.k = _operand(torch, "k", k, device, dt, (B, Lk, Hk, D))
-    a.v = _operand(torch, "v", v, device, dt, (B, Lk, Hk, D))
-    a.q_stride_b, a.q_stride_t, a.q_stride_h, _ = q.stride()
-    a.k_stride_b, a.k_stride_t, a.k_stride_h, _ = k.stride()
-    a.v_stride_b, a.v_stride_t, a.v_stride_h, _ = v.stride()
-    if q_lens is not None:
-        a.q_lens = _operand(torch, "q_lens", q_lens, device, torch.int32, (B,))
-    if k_lens is not None:
-        a.k_lens = _operand(torch, "k_lens", k_lens, device, torch.int32, (B,))
+    B, Lq, Hq, D = _sized(torch, "q", q, 4, "[B, Lq, heads, D]")
+    _, Lk, Hk, _ = _sized(torch, "k", k, 4, "[B, Lk, heads, D]")
+    dt, code, big = q.dtype, _type(torch, q), 2**31 - 1
+    left, right = window
+    left, right, sinks = max(-1, min(int(left), big)), max(-1, min(int(right), big)), min(int(sinks), big)
+    scale = float(scale) if scale is not None else D ** -0.5 if D > 0 else 0.0
+    pq = _operand(torch, "q", q, device, dt, (B, Lq, Hq, D))
+    pk, pv = _operand(torch, "k", k, device, dt, (B, Lk, Hk, D)), _operand(torch, "v", v, device, dt, (B, Lk, Hk, D))
+    pql = None if q_lens is None else _operand(torch, "q_lens", q_lens, device, torch.int32, (B,))
+    pkl = None if k_lens is None else _operand(torch, "k_lens", k_lens, device, torch.int32, (B,))
     if out is None:
         out = torch.empty((B, Lq, Hq, D), dtype=dt, device=device)
-    a.o = _operand(torch, "out", out, device, dt, (B, Lq, Hq, D))
-    a.o_stride_b, a.o_stride_t, a.o_stride_h, _ = out.stride()
-    return a, out
+        po = out.data_ptr()
+    else:
+        po = _operand(torch, "out", out, device, dt, (B, Lq, Hq, D))
+    return lib.BxAttentionArgs(code, B, Lq, Lk, Hq, Hk, D, left, right, sinks, scale, 0, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                               *out.stride()[:3], pq, pk, pv, po, pql, pkl, None, 0), out

@@ -286,6 +286,11 @@ class Context:
     def _stream(self):
         return C.c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
 
+    def _raw_stream(self):
+        """the same without building a Stream object, where torch offers it (a microsecond that short calls notice)"""
+        raw = getattr(self.torch._C, "_cuda_getCurrentRawStream", None)
+        return C.c_void_p(raw(self.device)) if raw is not None else self._stream()
+
     def _dev(self, a, dtype):
         t = self.torch
         if isinstance(a, t.Tensor):
@@ -372,7 +377,7 @@ class Context:
         "relu", "gelu", "silu".  m_dev: device int32 count of the rows in use (the others are left as they are in `out`)."""
         from . import dense
         args, out = dense.linear_args(self.torch, self.tdevice, x, weight, bias, act, residual, out, m_dev)
-        _chk(self.lib.bx_linear(self.handle, self._stream(), C.byref(args)), "bx_linear")
+        _chk(self.lib.bx_linear(self.handle, self._raw_stream(), C.byref(args)), "bx_linear")
         return out
 
     def qk_norm_rope(self, q, k, pos, freqs, sections, norm="rms", eps=1e-6, q_weight=None, k_weight=None, pairs="half", q_out=None,
@@ -383,7 +388,7 @@ class Context:
         from . import dense
         args, q_out, k_out = dense.qk_norm_rope_args(self.torch, self.tdevice, q, k, pos, freqs, sections, norm, eps, q_weight, k_weight, pairs,
                                                      q_out, k_out, m_dev)
-        _chk(self.lib.bx_qk_norm_rope(self.handle, self._stream(), C.byref(args)), "bx_qk_norm_rope")
+        _chk(self.lib.bx_qk_norm_rope(self.handle, self._raw_stream(), C.byref(args)), "bx_qk_norm_rope")
         return q_out, k_out
 
     def attention(self, q, k, v, scale=None, window=(-1, -1), sinks=0, q_lens=None, k_lens=None, out=None):
@@ -396,7 +401,7 @@ class Context:
         if need > 0:
             ws = self.torch.empty(need, dtype=self.torch.uint8, device=self.tdevice)
             args.workspace, args.workspace_bytes = ws.data_ptr(), need
-        _chk(self.lib.bx_attention(self.handle, self._stream(), C.byref(args)), "bx_attention")
+        _chk(self.lib.bx_attention(self.handle, self._raw_stream(), C.byref(args)), "bx_attention")
         return out
 
     # ---------------------------------------------------------------- pre-processing
