@@ -51,6 +51,22 @@ template <class T> __device__ __forceinline__ bxf4 bx_mma16(bxi4 a, bxi4 b, bxf4
     }
 }
 
+// eight floats as the sum of three bf16 operands: each plane holds the nearest bf16 to what the ones before it left
+__device__ __forceinline__ void bx_planes(const float* e, bxi4& p0, bxi4& p1, bxi4& p2)
+{
+    bx_bf16 a[8], b[8], c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        a[j] = (bx_bf16)e[j];
+        const float r = e[j] - (float)a[j];
+        b[j] = (bx_bf16)r;
+        c[j] = (bx_bf16)(r - (float)b[j]);
+    }
+    __builtin_memcpy(&p0, a, 16);
+    __builtin_memcpy(&p1, b, 16);
+    __builtin_memcpy(&p2, c, 16);
+}
+
 // elements [k, k + CH) of a row of `n` elements as one chunk; what lies at or behind n is zero and is not read
 template <class T, bool ALIGNED> __device__ __forceinline__ bxi4 bx_load_chunk(const T* __restrict__ row, int k, int n)
 {

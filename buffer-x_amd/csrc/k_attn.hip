@@ -65,13 +65,19 @@ __device__ __forceinline__ float other_half(float v)
 //
 // The reference value m of a row is a maximum that may lag: the weights are 2^((s - m) c) and m follows only when a score exceeds it by
 // more than 2^8 would allow -- rows of like scores rescale O once instead of every few tiles.  O and l belong to the same m at all times.
-template <class T, int DP>
+//
+// NP = 3 (f32 tiles): every operand is the sum of three bf16 numbers, a = a0 + a1 + a2 (8 + 8 + 8 bits, each the nearest to what is left: all 24 bits
+// are there).  Six of the nine products are multiplied, the smallest first; the three that are left out are below 2^-26 of a b, less
+// than the rounding of one f32 product.  Six bf16 matrix instructions take 3/8 of the time of the f32 ones they stand for, and the vector
+// unit works beside them, which it does not beside f32 ones: 524 -> 352 us for two clouds of 5000 keypoints, 8 heads of 32.  Infinities leave
+// the planes as NaN; a wave whose O is not all numbers redoes its rows in plain f32 (exact_rows).
+template <class T, int DP, int NP = 1>
 struct Rows {
     static constexpr int CH = BxElem<T>::CH, CPR = DP / CH, ND = DP / 32;
     // f16 weights are held times 2^7: with the 2^8 above they stay below 2^16 and the smallest keep their digits (O and l alike)
     static constexpr float BIAS = __is_same(T, bx_f16) ? 7.0f : 0.0f;
     bxf16 o[ND];
-    bxi4 fq[CPR / 2];
+    bxi4 fq[NP][CPR / 2];
     float m, thr, mb, l;
     bool edge;                                               // of the wave
     int lane, lr, h;
@@ -130,7 +136,18 @@ struct Rows {
 
     // the weights as second operands: registers of S^T as they are (f32), or rounded to the type of V -- half a step each, as V's own
     // values carry
-    struct Weights { bxf16 s[sizeof(T) == 4 ? 2 : 1]; bxi4 f[sizeof(T) == 4 ? 1 : 4]; };
+    struct Weights { bxf16 s[sizeof(T) == 4 ? 2 : 1]; bxi4 f[NP][sizeof(T) == 4 ? 1 : 4]; };
+    static constexpr int PLANE = BN * CPR;                   // chunks of a plane of K or V in LDS
+
+    static __device__ __forceinline__ bxf16 mma_planes(const bxi4* a, bxi4 b0, bxi4 b1, bxi4 b2, bxf16 acc)
+    {
+        acc = bx_mma32<T>(a[2], b0, acc);
+        acc = bx_mma32<T>(a[0], b2, acc);
+        acc = bx_mma32<T>(a[1], b1, acc);
+        acc = bx_mma32<T>(a[1], b0, acc);
+        acc = bx_mma32<T>(a[0], b1, acc);
+        return bx_mma32<T>(a[0], b0, acc);
+    }
 
     // acc += V^T P^T for dimensions 32 t ..
     __device__ __forceinline__ bxf16 weigh(const bxi4* sv, const Weights& w, int t, bxf16 acc) const
@@ -142,12 +159,20 @@ struct Rows {
                 for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(vfloat(sv, t, k2, i), w.s[k2][i], acc, 0, 0, 0);
         } else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) acc = bx_mma32<T>(vfrag(sv, t, u), w.f[u], acc);
+            for (int u = 0; u < 4; ++u) {
+                if constexpr (NP == 1) acc = bx_mma32<T>(vfrag(sv, t, u), w.f[0][u], acc);
+                else {
+                    bxi4 v[NP];
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) v[n] = vfrag(sv + n * PLANE, t, u);
+                    acc = mma_planes(v, w.f[0][u], w.f[1][u], w.f[2][u], acc);
+                }
+            }
         }
         return acc;
     }
 
-    // S^T of a tile: key(k2, c) is the operand of K for chunk pair c of block k2
+    // S^T of a tile: key(n, k2, c) is the operand of K for chunk pair c of block k2 (of plane n)
     struct Scores { bxf16 s[2]; };
     template <class Key> __device__ __forceinline__ void score(const Key& key, Scores& x) const
     {
@@ -156,17 +181,38 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < 16; ++i) x.s[k2][i] = 0.0f;
 #pragma unroll
-            for (int c2 = 0; c2 < CPR / 2; ++c2) x.s[k2] = bx_mma32<T>(key(k2, c2), fq[c2], x.s[k2]);
+            for (int c2 = 0; c2 < CPR / 2; ++c2) {
+                if constexpr (NP == 1) x.s[k2] = bx_mma32<T>(key(0, k2, c2), fq[0][c2], x.s[k2]);
+                else {
+                    bxi4 k[NP];
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) k[n] = key(n, k2, c2);
+                    x.s[k2] = mma_planes(k, fq[0][c2], fq[1][c2], fq[2][c2], x.s[k2]);
+                }
+            }
         }
     }
-    // a tile on the edge of the mask: sees(j) says whether this lane's row sees the key that is j behind the lane's first
-    template <class See> __device__ __forceinline__ void hide(Scores& x, const See& sees)
+    // a tile on the edge of the mask: this lane's row sees the keys [lo, hi) and those before sink, counted from the lane's first key.  Away
+    // from the first keys one unsigned comparison tells.
+    __device__ __forceinline__ void hide(Scores& x, int lo, int hi, int sink, bool first)
     {
         edge = true;
+        if (first) {
 #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2)
+            for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x.s[k2][i] = sees(32 * k2 + 8 * (i / 4) + i % 4) ? x.s[k2][i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) {
+                    const int j = 32 * k2 + 8 * (i / 4) + i % 4;
+                    x.s[k2][i] = j < hi && (j >= lo || j < sink) ? x.s[k2][i] : -INFINITY;
+                }
+        } else {
+            lo = max(lo, -(1 << 20));                        // the distances below stay inside 32 bits
+            const unsigned n = (unsigned)max(0, min(hi, 1 << 20) - lo);
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x.s[k2][i] = (unsigned)(32 * k2 + 8 * (i / 4) + i % 4 - lo) < n ? x.s[k2][i] : -INFINITY;
+        }
     }
     // the rows' reference values follow where the tile's scores are too far above them
     __device__ __forceinline__ void settle(const Scores& x, float c, float slack)
@@ -205,10 +251,16 @@ struct Rows {
         else {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                T e[8];
+                float e[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = (T)x.s[u / 2][8 * (u % 2) + j];
-                __builtin_memcpy(&w.f[u], e, 16);
+                for (int j = 0; j < 8; ++j) e[j] = x.s[u / 2][8 * (u % 2) + j];
+                if constexpr (NP == 3) bx_planes(e, w.f[0][u], w.f[1][u], w.f[2][u]);
+                else {
+                    T f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = (T)e[j];
+                    __builtin_memcpy(&w.f[0][u], f, 16);
+                }
             }
         }
     }
@@ -216,7 +268,7 @@ struct Rows {
     {
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
-            if constexpr (sizeof(T) == 4) {
+            if constexpr (sizeof(T) == 4 || NP == 3) {
                 // f32 sums a tile by itself first: fewer roundings at the size of O
                 bxf16 a;
 #pragma unroll
@@ -236,7 +288,7 @@ struct Rows {
         for (int t = 0; t < ND; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) z = fmaf(o[t][i], 0.0f, z);
-        return edge && __any(z != z);
+        return (edge || NP == 3) && __any(z != z);
     }
 };
 
@@ -292,18 +344,31 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
 }
 
 // DIRECT: 16-byte aligned rows and whole chunks go from memory straight into LDS, two buffers deep; others through registers.
+template <class T> struct Halves { using type = T; };
+template <> struct Halves<float> { using type = bx_bf16; };
+
+// elements [k, k + 8) of a row of n floats
+__device__ __forceinline__ void load8(const float* __restrict__ row, int k, int n, float* e)
+{
+    const bxi4 a = bx_load_chunk<float, false>(row, k, n), b = bx_load_chunk<float, false>(row, k + 4, n);
+    __builtin_memcpy(e, &a, 16);
+    __builtin_memcpy(e + 4, &b, 16);
+}
+
 constexpr int waves_of(int bytes, int DP, bool direct)
 {
-    const int w = (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (bytes == 4 ? 1 : 0) - (direct ? 0 : 1);      // without spills in the loop
-    return w < 1 ? 1 : w;
+    if (bytes == 4) return DP == 32 ? 3 : DP == 64 ? 2 : 1;
+    return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (direct ? 0 : 1);             // without spills in the loop
 }
 template <class T, int DP, int NW, bool DIRECT>
 __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn_kernel(AttnK p)
 {
-    constexpr int CH = BxElem<T>::CH, CPR = DP / CH, NT = NW * 64, LD = BN * CPR / NT;
+    constexpr bool F32 = sizeof(T) == 4;
+    static_assert(!(F32 && DIRECT), "f32 is taken apart on its way into LDS");
+    constexpr int CH = 8, CPR = DP / CH, NT = NW * 64, LD = BN * CPR / NT;   // chunks as they lie in LDS: 8 halves
     static_assert(BN * CPR % NT == 0, "every thread stages the same number of chunks");
-    __shared__ bxi4 sk0[BN * CPR], sv0[BN * CPR], sk1[DIRECT ? BN * CPR : 1], sv1[DIRECT ? BN * CPR : 1];
-    using R_ = Rows<T, DP>;
+    using R_ = Rows<typename Halves<T>::type, DP, F32 ? 3 : 1>;
+    __shared__ bxi4 sk0[(F32 ? 3 : 1) * BN * CPR], sv0[(F32 ? 3 : 1) * BN * CPR], sk1[DIRECT ? BN * CPR : 1], sv1[DIRECT ? BN * CPR : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = (int)bx_xcd_order<16>(blockIdx.x, gridDim.x);
     const int split = id % p.nsplit; id /= p.nsplit;
@@ -333,7 +398,13 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
     {
         const T* qr = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
 #pragma unroll
-        for (int c = 0; c < CPR / 2; ++c) w.fq[c] = bx_load_chunk<T, DIRECT>(qr, (2 * c + h) * CH, p.D);
+        for (int c = 0; c < CPR / 2; ++c) {
+            if constexpr (F32) {
+                float e[8];
+                load8(qr, (2 * c + h) * CH, p.D, e);
+                bx_planes(e, w.fq[0][c], w.fq[1][c], w.fq[2][c]);
+            } else w.fq[0][c] = bx_load_chunk<T, DIRECT>(qr, (2 * c + h) * CH, p.D);
+        }
     }
     const float slack = 8.0f / p.c;
 
@@ -341,8 +412,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
     const auto hide = [&](typename R_::Scores& x, int t) __attribute__((always_inline)) {
         const int j0 = base_of(t);
         if (j0 + BN <= w_hi0 && (j0 >= w_lo1 || j0 + BN <= p.sinks)) return;
-        const int a_hi = hi - j0 - 4 * h, a_lo = lo - j0 - 4 * h, a_sink = p.sinks - j0 - 4 * h;
-        w.hide(x, [&](int j) { return j < a_hi && (j >= a_lo || j < a_sink); });
+        w.hide(x, lo - j0 - 4 * h, hi - j0 - 4 * h, p.sinks - j0 - 4 * h, j0 < p.sinks);
     };
     const auto unseen = [&](int t) { const int j0 = base_of(t); return !wave_live || j0 >= w_hi1 || (j0 + BN <= w_lo0 && j0 >= p.sinks); };
 
@@ -378,60 +448,88 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
         const auto load_v = [&](int t) __attribute__((always_inline)) { load(vb, p.v_st, vs, vo, cv, (t - t0) & 1 ? sv1 : sv0, t); };
         const auto score = [&](typename R_::Scores& x, int t) __attribute__((always_inline)) {
             const bxi4* sk = (t - t0) & 1 ? sk1 : sk0;
-            w.score([&](int k2, int c) { return w.kfrag(sk, k2, c); }, x);
+            w.score([&](int, int k2, int c) { return w.kfrag(sk, k2, c); }, x);
         };
-        // One step: the weights of tile t (the vector unit) while the scores of tile t + 1 are multiplied (the matrix unit), then the sums
-        // of tile t.  K runs one tile ahead of V, and both are loaded one step before they are read.
-        const auto step = [&](typename R_::Scores& now, typename R_::Scores& next, int t) __attribute__((always_inline)) {
-            __syncthreads();
-            if (t + 2 < t1) load_k(t + 2);
-            load_v(t + 1);
-            typename R_::Weights u;
-            score(next, t + 1);
-            w.weights(now, p.c, u);
-            w.add((t - t0) & 1 ? sv1 : sv0, u);
-            hide(next, t + 1);
-            w.settle(next, p.c, slack);
-        };
-        const auto finish = [&](typename R_::Scores& now) __attribute__((always_inline)) {
-            __syncthreads();
-            typename R_::Weights u;
-            w.weights(now, p.c, u);
-            w.add((t1 - 1 - t0) & 1 ? sv1 : sv0, u);
-        };
-        if (t0 < t1) {
-            typename R_::Scores a, b2;
-            load_k(t0);
-            __syncthreads();
-            if (t0 + 1 < t1) load_k(t0 + 1);
-            load_v(t0);
-            score(a, t0);
-            hide(a, t0);
-            w.settle(a, p.c, slack);
-            int t = t0;
-            for (; t + 2 < t1; t += 2) {
-                step(a, b2, t);
-                step(b2, a, t + 1);
+        if constexpr (DP == 128) {
+            // One step: the weights of tile t (the vector unit) while the scores of tile t + 1 are multiplied (the matrix unit), then the sums
+            // of tile t.  K runs one tile ahead of V, and both are loaded one step before they are read.
+            const auto step = [&](typename R_::Scores& now, typename R_::Scores& next, int t) __attribute__((always_inline)) {
+                __syncthreads();
+                if (t + 2 < t1) load_k(t + 2);
+                load_v(t + 1);
+                typename R_::Weights u;
+                score(next, t + 1);
+                w.weights(now, p.c, u);
+                w.add((t - t0) & 1 ? sv1 : sv0, u);
+                hide(next, t + 1);
+                w.settle(next, p.c, slack);
+            };
+            const auto finish = [&](typename R_::Scores& now) __attribute__((always_inline)) {
+                __syncthreads();
+                typename R_::Weights u;
+                w.weights(now, p.c, u);
+                w.add((t1 - 1 - t0) & 1 ? sv1 : sv0, u);
+            };
+            if (t0 < t1) {
+                typename R_::Scores a, b2;
+                load_k(t0);
+                __syncthreads();
+                if (t0 + 1 < t1) load_k(t0 + 1);
+                load_v(t0);
+                score(a, t0);
+                hide(a, t0);
+                w.settle(a, p.c, slack);
+                int t = t0;
+                for (; t + 2 < t1; t += 2) {
+                    step(a, b2, t);
+                    step(b2, a, t + 1);
+                }
+                if (t + 1 < t1) {
+                    step(a, b2, t);
+                    finish(b2);
+                } else finish(a);
             }
-            if (t + 1 < t1) {
-                step(a, b2, t);
-                finish(b2);
-            } else finish(a);
+        } else {
+            // small heads: the vector unit has most of the work, and waves that do not see a tile leave it out
+            if (t0 < t1) { load_k(t0); load_v(t0); }
+            for (int t = t0; t < t1; ++t) {
+                __syncthreads();
+                if (t + 1 < t1) { load_k(t + 1); load_v(t + 1); }
+                if (unseen(t)) continue;
+                typename R_::Scores x;
+                typename R_::Weights u;
+                score(x, t);
+                hide(x, t);
+                w.settle(x, p.c, slack);
+                w.weights(x, p.c, u);
+                w.add((t - t0) & 1 ? sv1 : sv0, u);
+            }
         }
     } else {
-        bxi4 rk[LD], rv[LD];
-        const bxi4 zero = {0, 0, 0, 0};
+        // through registers: keys behind the sequence become zeros, f32 comes apart into its planes
+        constexpr int RW = F32 ? 2 : 1;
+        bxi4 rk[LD][RW], rv[LD][RW];
         const auto fetch = [&](int t) {
             const int j0 = base_of(t);
 #pragma unroll
             for (int i = 0; i < LD; ++i) {
                 const int e = tid + i * NT, key = j0 + e / CPR, d = e % CPR * CH;
-                rk[i] = rv[i] = zero;
-                if (key < sp.kl) {
-                    rk[i] = bx_load_chunk<T, false>(kb + (long long)key * p.k_st, d, p.D);
-                    rv[i] = bx_load_chunk<T, false>(vb + (long long)key * p.v_st, d, p.D);
+#pragma unroll
+                for (int j = 0; j < RW; ++j) {
+                    rk[i][j] = rv[i][j] = (bxi4){0, 0, 0, 0};
+                    if (key < sp.kl) {
+                        rk[i][j] = bx_load_chunk<T, false>(kb + (long long)key * p.k_st, d + j * BxElem<T>::CH, p.D);
+                        rv[i][j] = bx_load_chunk<T, false>(vb + (long long)key * p.v_st, d + j * BxElem<T>::CH, p.D);
+                    }
                 }
             }
+        };
+        const auto put = [&](bxi4* to, const bxi4* r) {
+            if constexpr (F32) {
+                float e[8];
+                __builtin_memcpy(e, r, 32);
+                bx_planes(e, to[0], to[R_::PLANE], to[2 * R_::PLANE]);
+            } else *to = *r;
         };
         if (t0 < t1) fetch(t0);
         for (int t = t0; t < t1; ++t) {
@@ -439,15 +537,15 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
 #pragma unroll
             for (int i = 0; i < LD; ++i) {
                 const int e = tid + i * NT, key = e / CPR, c = e % CPR;
-                sk0[key * CPR + (c ^ R_::kswz(key))] = rk[i];
-                sv0[key * CPR + (c ^ R_::vswz(key))] = rv[i];
+                put(&sk0[key * CPR + (c ^ R_::kswz(key))], rk[i]);
+                put(&sv0[key * CPR + (c ^ R_::vswz(key))], rv[i]);
             }
             __syncthreads();
             if (t + 1 < t1) fetch(t + 1);
             if (unseen(t)) continue;
             typename R_::Scores x;
             typename R_::Weights u;
-            w.score([&](int k2, int c) { return w.kfrag(sk0, k2, c); }, x);
+            w.score([&](int n, int k2, int c) { return w.kfrag(sk0 + n * R_::PLANE, k2, c); }, x);
             hide(x, t);
             w.settle(x, p.c, slack);
             w.weights(x, p.c, u);
@@ -522,7 +620,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
     {
         const T* qr = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
 #pragma unroll
-        for (int c = 0; c < CPR / 2; ++c) w.fq[c] = bx_load_chunk<T, false>(qr, (2 * c + h) * CH, p.D);
+        for (int c = 0; c < CPR / 2; ++c) w.fq[0][c] = bx_load_chunk<T, false>(qr, (2 * c + h) * CH, p.D);
     }
     const float slack = 8.0f / p.c;
     if (p.D < DP) {
@@ -547,11 +645,10 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
             if (cv < p.D) bx_load_lds16(vr, sv + i * 64);
         }
         const bool masked = !(j0 + BN <= w_hi0 && (j0 >= w_lo1 || j0 + BN <= p.sinks)) || sp.R < 32;
-        const int a_hi = hi - j0 - 4 * h, a_lo = lo - j0 - 4 * h, a_sink = p.sinks - j0 - 4 * h;
         typename R_::Scores x;
         typename R_::Weights u;
-        w.score([&](int k2, int c) { return fk[k2][c]; }, x);
-        if (masked) w.hide(x, [&](int j) { return j < a_hi && (j >= a_lo || j < a_sink); });
+        w.score([&](int, int k2, int c) { return fk[k2][c]; }, x);
+        if (masked) w.hide(x, lo - j0 - 4 * h, hi - j0 - 4 * h, p.sinks - j0 - 4 * h, j0 < p.sinks);
         w.settle(x, p.c, slack);
         w.weights(x, p.c, u);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's V is there
@@ -660,6 +757,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
 
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
+// waves of a workgroup (32 rows each).  Small heads of halves take two: their tiles are short work and rows come in few (1500 patches of 2 heads
+// over 140 positions, f16: 39 us, 45 by four waves); four share more of the staging of everything else (clouds f32: 324 us, 425 by two).
+constexpr int group_of(int bytes, int DP) { return bytes == 2 && DP == 32 ? 2 : 4; }
+
 struct Shape { int DP, tiles_r, nsplit; bool rows; };
 
 // whether rows of 16-byte aligned whole chunks let K and V skip the registers
@@ -678,7 +779,7 @@ Shape shape_of(int n_cu, const bx_attention_args& a)
     s.DP = padded(a.D);
     const long long R = (long long)a.Lq * (a.Hq / a.Hk);
     s.rows = R <= 32 && direct_of(a);
-    s.tiles_r = (int)((R + 127) / 128);
+    s.tiles_r = (int)((R + 32 * group_of(a.dtype == BX_TYPE_F32 ? 4 : 2, s.DP) - 1) / (32 * group_of(a.dtype == BX_TYPE_F32 ? 4 : 2, s.DP)));
     const long long base = (long long)s.tiles_r * a.Hk * a.B;
     long long keys = a.Lk;
     if (a.left >= 0 && a.right >= 0) {
@@ -691,6 +792,11 @@ Shape shape_of(int n_cu, const bx_attention_args& a)
     long long n = base > 0 ? 2LL * n_cu / base : 1;
     if (n > (tiles + 3) / 4) n = (tiles + 3) / 4;
     if (n > 128) n = 128;
+    // A few workgroups a compute unit, unevenly: two halves even them out (two clouds of 5000 keypoints f32, 640 workgroups: 352 -> 323 us).
+    if (n <= 1 && base < 4LL * n_cu && tiles >= 32) {
+        const auto worst = [n_cu](long long g) { return (double)((g + n_cu - 1) / n_cu) * n_cu / (double)g; };
+        if (worst(base) - worst(2 * base) > 0.12) n = 2;
+    }
     s.nsplit = n < 1 ? 1 : (int)n;
     return s;
 }
@@ -704,10 +810,12 @@ int64_t bytes_of(const Shape& s, const bx_attention_args& a)
 template <class T, int DP>
 int launch(hipStream_t s, const AttnK& k, bool rows_form, bool direct)
 {
+    constexpr int G = group_of(sizeof(T), DP);
     const unsigned grid = (unsigned)((long long)k.tiles_r * k.Hk * k.B * k.nsplit);
     if (rows_form) attn_rows_kernel<T, DP><<<grid, 256, 0, s>>>(k);
-    else if (direct) attn_kernel<T, DP, 4, true><<<grid, 256, 0, s>>>(k);
-    else attn_kernel<T, DP, 4, false><<<grid, 256, 0, s>>>(k);
+    else if constexpr (sizeof(T) == 4) attn_kernel<T, DP, G, false><<<grid, G * 64, 0, s>>>(k);
+    else if (direct) attn_kernel<T, DP, G, true><<<grid, G * 64, 0, s>>>(k);
+    else attn_kernel<T, DP, G, false><<<grid, G * 64, 0, s>>>(k);
     BX_LAUNCH_CHECK();
     if (k.nsplit > 1) {
         constexpr int SG = 32 * 8 / (DP / 4) > 8 ? 8 : 32 * 8 / (DP / 4);
