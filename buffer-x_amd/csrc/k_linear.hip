@@ -289,6 +289,127 @@ __global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(Linear
     else put_rows<T, TM, TN, BX_ACT_SILU>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
 }
 
+// f32 by bf16 planes: every operand is the sum of three bf16 numbers, a = a0 + a1 + a2 (8 + 8 + 8 bits, each the nearest to what is left: all 24
+// bits are there), taken apart on the way into LDS.  Six of the nine products are multiplied, the smallest first; the three left out are
+// below 2^-26 of a b, less than the rounding of one f32 product.  The six bf16 matrix instructions take 3/8 of the time of the f32 ones.
+// An infinity leaves the planes as NaN: results that are not finite are summed again, in plain f32.
+template <int BM, int BN, int WGM, int WGN>
+__global__ __launch_bounds__(WGM * WGN * 64) void linear_planes_kernel(LinearK p)
+{
+    using T = float;
+    constexpr int NW = WGM * WGN, NT = NW * 64, BK = 32, TM = BM / WGM / 32, TN = BN / WGN / 32;
+    constexpr int LX = BM * 4 / NT, LW = BN * 4 / NT, PX = BM * 4, PW = BN * 4, BUF = 3 * (PX + PW);      // pieces of 8 elements: a thread's, a plane's
+    constexpr int PUT = NW * 32 * (TN * 32 + 4) / 4;
+    __shared__ bxi4 lds[PUT > 2 * BUF ? PUT : 2 * BUF];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int id = (int)bx_xcd_order<32>(blockIdx.x, gridDim.x), gsize = 8 * p.tiles_n, first = id / gsize * 8, gm = min(8, p.tiles_m - first);
+    const int m0 = (first + id % gsize % gm) * BM, n0 = (id % gsize / gm) * BN;
+    int M = p.M;
+    if (p.m_dev) { const int live = *p.m_dev; M = live < M ? live : M; }
+    if (m0 >= M) return;
+    const T* x = (const T*)p.x + (long long)m0 * p.ldx;
+    const T* w = (const T*)p.w + (long long)n0 * p.ldw;
+    const int last_m = M - 1 - m0, last_n = p.N - 1 - n0;
+
+    bxf16 acc[TN][TM];
+#pragma unroll
+    for (int a = 0; a < TN; ++a)
+#pragma unroll
+        for (int b = 0; b < TM; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.0f;
+    const int wm = (wave / WGN) * TM * 32, wn = (wave % WGN) * TN * 32, lr = lane & 31, h = lane >> 5;
+    // rows of 64 bytes: four of them cover the banks, chunk c of row r sits at c ^ (r / 4 % 4)
+    const int x_at = (wm + lr) * 64 + ((h ^ (lr >> 2 & 3)) * 16), w_at = 3 * PX * 16 + (wn + lr) * 64 + ((h ^ (lr >> 2 & 3)) * 16);
+
+    bxi4 rx[LX][2], rw[LW][2];
+    const auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            const int e = tid + i * NT;
+            const T* row = x + (long long)min(e >> 2, last_m) * p.ldx;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) rx[i][j] = bx_load_chunk<T, false>(row, k0 + (e & 3) * 8 + j * 4, p.K);
+        }
+#pragma unroll
+        for (int i = 0; i < LW; ++i) {
+            const int e = tid + i * NT;
+            const T* row = w + (long long)min(e >> 2, last_n) * p.ldw;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) rw[i][j] = bx_load_chunk<T, false>(row, k0 + (e & 3) * 8 + j * 4, p.K);
+        }
+    };
+    const auto put = [&](bxi4* plane, int stride, int e, const bxi4* r) {
+        float f[8];
+        __builtin_memcpy(f, r, 32);
+        bxi4* to = plane + (e >> 2) * 4 + ((e & 3) ^ (e >> 4 & 3));
+        bx_planes(f, to[0], to[stride], to[2 * stride]);
+    };
+    const auto stage = [&](bxi4* buf) {
+#pragma unroll
+        for (int i = 0; i < LX; ++i) put(buf, PX, tid + i * NT, rx[i]);
+#pragma unroll
+        for (int i = 0; i < LW; ++i) put(buf + 3 * PX, PW, tid + i * NT, rw[i]);
+    };
+    const auto multiply = [&](const bxi4* buf) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            bxi4 fx[TM][3], fw[TN][3];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+#pragma unroll
+                for (int b = 0; b < TM; ++b) fx[b][n] = *(const bxi4*)((const char*)buf + (x_at ^ (c * 32)) + n * PX * 16 + b * 32 * 64);
+#pragma unroll
+                for (int a = 0; a < TN; ++a) fw[a][n] = *(const bxi4*)((const char*)buf + (w_at ^ (c * 32)) + n * PW * 16 + a * 32 * 64);
+            }
+            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+            for (int q = 0; q < 6; ++q)
+#pragma unroll
+                for (int a = 0; a < TN; ++a)
+#pragma unroll
+                    for (int b = 0; b < TM; ++b) acc[a][b] = bx_mma32<bx_bf16>(fw[a][PA[q]], fx[b][PB[q]], acc[a][b]);
+        }
+    };
+    const int steps = (p.K + BK - 1) / BK;
+    if (steps > 0) { fetch(0); stage(lds); }
+    for (int s = 0; s < steps; ++s) {
+        __syncthreads();
+        if (s + 1 < steps) fetch((s + 1) * BK);
+        multiply(lds + (s & 1) * BUF);
+        if (s + 1 < steps) stage(lds + (~s & 1) * BUF);
+    }
+
+    bool odd = false;
+#pragma unroll
+    for (int a = 0; a < TN; ++a)
+#pragma unroll
+        for (int b = 0; b < TM; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) odd |= !(fabsf(acc[a][b][i]) < INFINITY);
+    if (__any(odd)) {
+#pragma unroll
+        for (int a = 0; a < TN; ++a)
+#pragma unroll
+            for (int b = 0; b < TM; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(fabsf(acc[a][b][i]) < INFINITY)) {
+                        const T* xr = x + (long long)min(wm + b * 32 + lr, last_m) * p.ldx;
+                        const T* wr = w + (long long)min(wn + a * 32 + 8 * (i / 4) + 4 * h + i % 4, last_n) * p.ldw;
+                        float sum = 0.0f;
+                        for (int k = 0; k < p.K; ++k) sum = fmaf(xr[k], wr[k], sum);
+                        acc[a][b][i] = sum;
+                    }
+    }
+    __syncthreads();
+    float* mine = (float*)lds + wave * 32 * (TN * 32 + 4);
+    if (p.act == BX_ACT_NONE) put_rows<T, TM, TN, BX_ACT_NONE>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
+    else if (p.act == BX_ACT_RELU) put_rows<T, TM, TN, BX_ACT_RELU>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
+    else if (p.act == BX_ACT_GELU) put_rows<T, TM, TN, BX_ACT_GELU>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
+    else put_rows<T, TM, TN, BX_ACT_SILU>(p, acc, mine, lane, m0 + wm, n0 + wn, M);
+}
+
 // Few rows: one workgroup = 16 columns of y x 16 rows, its NW waves split K and meet in LDS.  Operands go from memory to the matrix
 // units directly: a wave reads 64 bytes of 16 rows of W per step, and W is read once per 16 rows of x.
 template <class T, int NW, bool ALIGNED>
@@ -346,6 +467,18 @@ int launch_tile(hipStream_t s, LinearK k, bool aligned)
     return BX_OK;
 }
 
+template <int BM, int BN, int WGM, int WGN>
+int launch_planes(hipStream_t s, LinearK k)
+{
+    k.tiles_n = (k.N + BN - 1) / BN;
+    k.tiles_m = (k.M + BM - 1) / BM;
+    const long long tiles = (long long)k.tiles_n * k.tiles_m;
+    if (tiles > 0x7fffffffLL || k.tiles_n > (1 << 27)) { bx_set_error("bx_linear: %lld tiles exceed one launch", tiles); return BX_ERR_ARG; }
+    linear_planes_kernel<BM, BN, WGM, WGN><<<(unsigned)tiles, WGM * WGN * 64, 0, s>>>(k);
+    BX_LAUNCH_CHECK();
+    return BX_OK;
+}
+
 template <class T>
 int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
 {
@@ -372,10 +505,17 @@ int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
         if (tiles(64, 32) <= n_cu) return launch_tile<T, 64, 32, 2, 1, 4>(s, k, aligned);
         if (tiles(64, 64) <= n_cu) return launch_tile<T, 64, 64, 2, 2, 2>(s, k, aligned);
     }
-    // Large outputs: halves want 256 x 256 (16384 x 4096 by K = 1024 with gelu 174 us; 175 by 128 x 128, 192 by 64 x 128), f32, whose
-    // matrix rate is a sixteenth, the smaller tiles' occupancy (10000 x 1024 by 1024: 171 us by 64 x 128, 195 by 64 x 64, 242 by 256 x 256).
-    if (sizeof(T) == 2 && tiles(256, 256) >= 2 * n_cu) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
-    if (k.N > 64 && tiles(64, 128) >= 4 * n_cu && k.K >= 256) return launch_tile<T, 64, 128, 2, 2>(s, k, aligned);
+    if constexpr (sizeof(T) == 2) {
+        // Large outputs want 256 x 256 (16384 x 4096 by K = 1024 bf16 with gelu: 174 us; 175 by 128 x 128, 192 by 64 x 128).
+        if (tiles(256, 256) >= 2 * n_cu) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
+        if (k.N > 64 && tiles(64, 128) >= 4 * n_cu && k.K >= 256) return launch_tile<T, 64, 128, 2, 2>(s, k, aligned);
+    } else if (k.K >= 128) {
+        // f32 by planes: 8192 x 4096 by 1024 361 us (442 by 64 x 128, 532 on the f32 units), 10000 x 1024 by 1024 150 us (177), 10000 x 256 by
+        // 256 20.4 us (23.3).  Shorter sums are bound by memory either way (700000 x 64 by 32: 62 us both).
+        if (tiles(128, 256) >= 3 * n_cu) return launch_planes<128, 256, 2, 4>(s, k);
+        if (k.N > 64 && tiles(64, 128) >= 4 * n_cu) return launch_planes<64, 128, 2, 2>(s, k);
+        return launch_planes<64, 64, 2, 2>(s, k);
+    }
     return launch_tile<T, 64, 64, 2, 2>(s, k, aligned);
 }
 

@@ -175,6 +175,21 @@ def test_linear_nonfinite_stays_in_its_row(ctx):
             assert bool(torch.isfinite(y[rest]).all())
 
 
+@pytest.mark.parametrize("M,N,K", [(3000, 400, 160), (9000, 1024, 256), (25000, 1100, 136)])
+def test_linear_f32_long_sums(ctx, M, N, K):
+    """f32 outputs large enough to be summed by planes: roundings as f32's, and rows with NaN, infinities or the largest numbers as f32 has them"""
+    rng = np.random.default_rng(K)
+    x, w = _rand(rng, (M, K), "f32"), _rand(rng, (N, K), "f32", K ** -0.5)
+    x[5] *= 1e30
+    x[6] *= 1e-30
+    x[9, 3], x[17, 1], x[23, 2], x[40] = float("nan"), float("inf"), -float("inf"), 0.0
+    x[31, 7] = torch.finfo(torch.float32).max
+    w[:, 7] *= 0.25                                          # |w| < 1: the products of the largest number stay finite
+    y = ctx.linear(x, w)
+    want, tol = _linear_ref(x, w, None, "none", None, "f32")
+    _within(y, want, tol, (M, N, K))
+
+
 def test_linear_far_rows(ctx):
     """row offsets past 2^31 elements"""
     ld = (1 << 30) + 8
@@ -437,6 +452,24 @@ def test_attention_extreme_scores(ctx, dt):
     k[:, :, 0] = -float("inf")
     got = ctx.attention(q, k, v, scale=1.0)
     assert bool(torch.isnan(got[:, :, 0]).all()) and bool(torch.isfinite(got[:, :, 1]).all())
+
+
+def test_attention_f32_infinite_and_large(ctx):
+    """f32 keys of -inf get no weight, values of +-inf reach the rows that see them, large and small values keep their digits"""
+    q, k, v = _attention_inputs("f32", 1, 90, 150, 2, 1, 32)
+    q = q.abs()
+    k[:, 40] = -float("inf")                                 # scores -inf in every row
+    v[:, :, :, 3] *= 1e30
+    v[:, :, :, 4] *= 1e-30
+    got = ctx.attention(q, k, v)
+    keep = [j for j in range(150) if j != 40]
+    want, tol = _attention_ref(q[0], k[0, keep], v[0, keep], 32 ** -0.5, -1, -1, 0, "f32")
+    _within(got[0], want, tol)
+    v[0, 60, 0, 5], v[0, 61, 0, 6], v[0, 62, 0, 6] = float("inf"), float("inf"), -float("inf")
+    got = _d(ctx.attention(q, k, v))[0]
+    assert bool((got[:, :, 5] == math.inf).all()) and bool(torch.isnan(got[:, :, 6]).all())
+    dims = [d for d in range(32) if d not in (5, 6)]
+    _within(got[:, :, dims], want[:, :, dims], tol[:, :, dims])
 
 
 def test_attention_zero_sizes(ctx):
