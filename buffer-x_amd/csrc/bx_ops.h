@@ -130,6 +130,14 @@ template <unsigned C> __device__ __forceinline__ unsigned bx_xcd_order(unsigned 
     return j / C * (8 * C) + x * C + j % C;
 }
 
+// a launch has fewer than 2^32 threads
+inline int bx_grid_check(const char* what, long long groups, int threads)
+{
+    if (groups * threads < 1LL << 32) return BX_OK;
+    bx_set_error("%s: %lld workgroups exceed one launch", what, groups);
+    return BX_ERR_ARG;
+}
+
 int bxk_linear(hipStream_t s, int n_cu, const bx_linear_args& a);
 int bxk_qk_norm_rope(hipStream_t s, int n_cu, const bx_qk_norm_rope_args& a);
 int64_t bxk_attention_workspace(int n_cu, const bx_attention_args& a);

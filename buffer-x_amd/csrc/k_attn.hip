@@ -859,9 +859,9 @@ int bxk_attention(hipStream_t s, int n_cu, const bx_attention_args& a)
         bx_set_error("bx_attention: workspace of %lld bytes, needs %lld (bx_attention_workspace)", (long long)a.workspace_bytes, (long long)need);
         return BX_ERR_STATE;
     }
-    if (((long long)sh.tiles_r * a.Hk * a.B) * sh.nsplit > 0x7fffffffLL || (long long)a.B * a.Lq * a.Hq > 0x7fffffffLL) {
-        bx_set_error("bx_attention: too many rows for one launch"); return BX_ERR_ARG;
-    }
+    // (joining has less than a workgroup per row)
+    if (bx_grid_check("bx_attention", (long long)sh.tiles_r * a.Hk * a.B * sh.nsplit, 256) != BX_OK ||
+        (sh.nsplit > 1 && bx_grid_check("bx_attention", (long long)a.B * a.Lq * a.Hq, 256) != BX_OK)) return BX_ERR_ARG;
     if (a.dtype == BX_TYPE_F32) return attention_of<float>(s, n_cu, a);
     if (a.dtype == BX_TYPE_F16) return attention_of<bx_f16>(s, n_cu, a);
     return attention_of<bx_bf16>(s, n_cu, a);

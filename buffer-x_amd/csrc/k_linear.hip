@@ -459,7 +459,7 @@ int launch_tile(hipStream_t s, LinearK k, bool aligned)
     k.tiles_n = (k.N + BN - 1) / BN;
     k.tiles_m = (k.M + BM - 1) / BM;
     const long long tiles = (long long)k.tiles_n * k.tiles_m;
-    if (tiles > 0x7fffffffLL || k.tiles_n > (1 << 27)) { bx_set_error("bx_linear: %lld tiles exceed one launch", tiles); return BX_ERR_ARG; }
+    if (bx_grid_check("bx_linear", tiles, KS * WGM * WGN * 64) != BX_OK) return BX_ERR_ARG;
     const long long far = (1LL << 31) / (256 * (long long)sizeof(T));
     if (aligned && k.ldx < far && k.ldw < far) linear_tile_kernel<T, BM, BN, WGM, WGN, KS, true><<<(unsigned)tiles, KS * WGM * WGN * 64, 0, s>>>(k);
     else linear_tile_kernel<T, BM, BN, WGM, WGN, KS, false><<<(unsigned)tiles, KS * WGM * WGN * 64, 0, s>>>(k);
@@ -473,7 +473,7 @@ int launch_planes(hipStream_t s, LinearK k)
     k.tiles_n = (k.N + BN - 1) / BN;
     k.tiles_m = (k.M + BM - 1) / BM;
     const long long tiles = (long long)k.tiles_n * k.tiles_m;
-    if (tiles > 0x7fffffffLL || k.tiles_n > (1 << 27)) { bx_set_error("bx_linear: %lld tiles exceed one launch", tiles); return BX_ERR_ARG; }
+    if (bx_grid_check("bx_linear", tiles, WGM * WGN * 64) != BX_OK) return BX_ERR_ARG;
     linear_planes_kernel<BM, BN, WGM, WGN><<<(unsigned)tiles, WGM * WGN * 64, 0, s>>>(k);
     BX_LAUNCH_CHECK();
     return BX_OK;
@@ -491,7 +491,7 @@ int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
     // by K = 2048 bf16 28 us, 9.0 by tiles.
     const long long pieces = tiles(16, 16);
     if (k.M <= 16 || pieces <= n_cu) {
-        if (pieces > 0x7fffffffLL) { bx_set_error("bx_linear: %lld pieces exceed one launch", pieces); return BX_ERR_ARG; }
+        if (bx_grid_check("bx_linear", pieces, 512) != BX_OK) return BX_ERR_ARG;
         k.tiles_n = (k.N + 15) / 16;
         if (aligned) linear_rows_kernel<T, 8, true><<<(unsigned)pieces, 512, 0, s>>>(k);
         else linear_rows_kernel<T, 8, false><<<(unsigned)pieces, 512, 0, s>>>(k);

@@ -214,6 +214,7 @@ int rope_of(hipStream_t s, int n_cu, const RopeK& k)
     if (k.pairs > 0 && tpb > 49152 / (8 * k.pairs)) tpb = 49152 / (8 * k.pairs);
     if (tpb < 1) tpb = 1;
     const unsigned grid = (unsigned)((k.T + tpb - 1) / tpb);
+    if (bx_grid_check("bx_qk_norm_rope", grid, 256) != BX_OK) return BX_ERR_ARG;
     switch (lpr) {
         case 1: return rope_launch<T, 1, N>(s, k, vec, (int)tpb, grid);
         case 2: return rope_launch<T, 2, N>(s, k, vec, (int)tpb, grid);

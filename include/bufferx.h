@@ -311,7 +311,7 @@ int bx_refine(bx_ctx *ctx, void *stream, const float *ss, const float *tt, const
  * Counts and lengths that depend on the data are device int32, read when the kernel runs and clamped to [0, the size given here];
  * rows at or behind them are neither read nor written.  Sizes of zero are answered without a launch.
  * Outputs must not overlap any input (exceptions are named) nor themselves: BX_ERR_ARG.  Results do not depend on the stream, on the
- * run or on other calls: the order of every sum is fixed by the sizes.  The calls keep no state and share none, so several may run at
+ * run or on other calls: the order of every sum is fixed by sizes, lengths and alignment.  The calls keep no state and share none, so several may run at
  * once, on one context too, and may be captured; the memory they are given must stay valid until they have run.  */
 #define BX_TYPE_F32 0
 #define BX_TYPE_F16 1
@@ -322,7 +322,9 @@ int bx_refine(bx_ctx *ctx, void *stream, const float *ss, const float *tt, const
 #define BX_ACT_SILU 3    /* v / (1 + exp(-v)) */
 
 /* y = act(x w^T + bias) + residual.  x [M][K], w [N][K], bias [N] (nullable), residual and y [M][N] (residual nullable; it may be y
- * itself, with the same stride).  M, N, K < 2^31.  m_dev (nullable): device count of the rows that are in use.            */
+ * itself, with the same stride).  M, N, K <= 2^30.  f32 sums of 128 terms and more run on the bf16 matrix units, every operand as three
+ * bf16 numbers that hold all its 24 bits (operands below 2^-100 keep fewer); where an infinity or NaN is among them they are
+ * summed again in plain f32.  m_dev (nullable): device count of the rows in use.                                               */
 typedef struct bx_linear_args {
     int32_t dtype, act;
     int64_t M, N, K;
@@ -333,7 +335,7 @@ typedef struct bx_linear_args {
 } bx_linear_args;
 int bx_linear(bx_ctx *ctx, void *stream, const bx_linear_args *args);
 
-/* q [T][Hq][D] and k [T][Hk][D] (either pointer nullable), every head row x of length D (1..256):
+/* q [T][Hq][D] and k [T][Hk][D] (either pointer nullable; T <= 2^30), every head row x of length D (1..256):
  *   y = x * w * n,   n = 1 (BX_NORM_NONE), 1 / sqrt(mean(x^2) + eps) (BX_NORM_RMS), 1 / max(|x|, eps) (BX_NORM_L2); w [D] nullable = 1
  *   then rotation pair p of axis a:  (y_i, y_j) -> (y_i cos t - y_j sin t, y_j cos t + y_i sin t),  t = pos[token][a] * freqs[p].
  * sections[a] = number of pairs of axis a (axes 1..4; the pairs of axis 0 come first, P = their sum, 2 P <= D); (i, j) = (p, p + P)
@@ -362,13 +364,16 @@ typedef struct bx_qk_norm_rope_args {
 } bx_qk_norm_rope_args;
 int bx_qk_norm_rope(bx_ctx *ctx, void *stream, const bx_qk_norm_rope_args *args);
 
-/* Attention: q, o [B][Lq][Hq][D], k, v [B][Lk][Hk][D], Hq a multiple of Hk (query head h reads key head h / (Hq / Hk)), D 1..128.
+/* Attention: q, o [B][Lq][Hq][D], k, v [B][Lk][Hk][D], Hq a multiple of Hk (query head h reads key head h / (Hq / Hk)), D 1..128,
+ * B Lq Hq and Lk < 2^30.
  *   o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys that query i of a batch entry sees:
  *   j < k_len,  j <= p_i + right (right >= 0),  j >= p_i - left (left >= 0) or j < sinks,      p_i = i + k_len - q_len
  * (the last query stands at the last key).  left / right < 0: no bound on that side.  A query that sees no key gets zeros; keys that it
- * does not see do not touch its result, whatever they hold, infinities and NaN included.  scale > 0 and finite.
+ * does not see do not touch its result, whatever they hold, infinities and NaN included.  scale in [2^-100, 2^100].
  * q_lens / k_lens: device int32 [B], nullable (Lq / Lk).
- * The softmax weights are rounded to the type of v before they are multiplied (f16 / bf16).
+ * The softmax weights are rounded to the type of v before they are multiplied (f16 / bf16); f32 as in bx_linear.  Rows that meet an
+ * infinity or NaN on the edge of their mask (f32: anywhere) are summed one by one: right, but
+ * hundreds of times slower, and rounded differently in the last place.
  * workspace: device memory of bx_attention_workspace(ctx, args) bytes (0: none needed; a host function of the sizes alone), aligned to 16 bytes,
  * used until the call has run and by no other call meanwhile; BX_ERR_STATE when it is too small.               */
 typedef struct bx_attention_args {

@@ -39,7 +39,7 @@ def test_linear_accepts(lib, kw):
 
 
 @pytest.mark.parametrize("kw,says", [
-    (dict(dtype=3), "type"), (dict(dtype=-1), "type"), (dict(act=4), "activation"), (dict(M=-1), "range"), (dict(K=2**31), "range"),
+    (dict(dtype=3), "type"), (dict(dtype=-1), "type"), (dict(act=4), "activation"), (dict(M=-1), "range"), (dict(K=2**31), "range"), (dict(M=2**30 + 1), "range"), (dict(K=2**30 + 1), "range"),
     (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"), (dict(ldx=-1), "stride"), (dict(ldy=7), "overlap"),
     (dict(ldx=2**50), "stride"), (dict(x=0x10001), "aligned"), (dict(m_dev=0x60002), "aligned"), (dict(y=0x10000), "overlaps"),
     (dict(y=0x20010), "overlaps"), (dict(y=0x30000), "overlaps"), (dict(residual=0x50002), "residual"), (dict(residual=0x50000, ldr=9), "residual"),
@@ -107,7 +107,8 @@ def test_attention_accepts(lib, kw):
 @pytest.mark.parametrize("kw,says", [
     (dict(dtype=3), "type"), (dict(D=0), "D="), (dict(D=129), "D="), (dict(Hq=3), "share"), (dict(Hk=0), "share"), (dict(Lk=-1), "range"),
     (dict(Lk=2**30), "range"), (dict(Lq=2**29, Hq=4), "range"), (dict(sinks=-1), "negative"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
-    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=None), "null"), (dict(k=None), "null"), (dict(o=None), "null"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=2.0**101), "scale"), (dict(scale=2.0**-101), "scale"),
+    (dict(q=None), "null"), (dict(k=None), "null"), (dict(o=None), "null"),
     (dict(v_stride_t=-1), "stride"), (dict(q=0x10001), "aligned"), (dict(k_lens=0x51002), "aligned"), (dict(workspace=0x60008, workspace_bytes=64), "aligned"),
     (dict(o_stride_h=7), "rows of o"), (dict(o_stride_b=0), "rows of o"), (dict(o=0x10000), "overlaps"), (dict(o=0x30010), "overlaps"),
     (dict(workspace=0x40000, workspace_bytes=64), "workspace"), (dict(workspace=0x20000, workspace_bytes=64), "workspace"), (dict(reserved=1), "reserved")])
