@@ -67,20 +67,34 @@ __device__ __forceinline__ void bx_planes(const float* e, bxi4& p0, bxi4& p1, bx
     __builtin_memcpy(&p2, c, 16);
 }
 
-// elements [k, k + CH) of a row of `n` elements as one chunk; what lies at or behind n is zero and is not read
-template <class T, bool ALIGNED> __device__ __forceinline__ bxi4 bx_load_chunk(const T* __restrict__ row, int k, int n)
+// elements [k, k + CH) of a row, all of which exist
+template <class T> __device__ __forceinline__ bxi4 bx_load_whole(const T* __restrict__ row, int k) { return reinterpret_cast<const BxAny16*>(row + k)->v; }
+
+// elements [k, k + CH) of a row of `n` elements as one chunk; what lies at or behind n is zero and is not read: the last chunk of a row is
+// loaded from where it still fits and shifted into place, rows shorter than a chunk go element by element
+template <class T> __device__ __forceinline__ bxi4 bx_load_chunk(const T* __restrict__ row, int k, int n)
 {
     constexpr int CH = BxElem<T>::CH;
-    if (k + CH <= n) {
-        if constexpr (ALIGNED) return *reinterpret_cast<const bxi4*>(row + k);
-        else return reinterpret_cast<const BxAny16*>(row + k)->v;
-    }
-    T e[CH];
+    if (n < CH) {
+        T e[CH];
 #pragma unroll
-    for (int j = 0; j < CH; ++j) e[j] = k + j < n ? row[k + j] : (T)0.0f;
-    bxi4 r;
-    __builtin_memcpy(&r, e, 16);
-    return r;
+        for (int j = 0; j < CH; ++j) e[j] = k + j < n ? row[k + j] : (T)0.0f;
+        bxi4 r;
+        __builtin_memcpy(&r, e, 16);
+        return r;
+    }
+    if (k >= n) return (bxi4){0, 0, 0, 0};
+    const int a = min(k, n - CH);
+    bxi4 v = reinterpret_cast<const BxAny16*>(row + a)->v;
+    if (k > a) {
+        typedef unsigned long long u2 __attribute__((ext_vector_type(2)));
+        u2 w = __builtin_bit_cast(u2, v);
+        const int s = (k - a) * (int)sizeof(T) * 8;          // 16 .. 112 bits
+        w[0] = s >= 64 ? w[1] >> (s - 64) : (w[0] >> s | w[1] << (64 - s));
+        w[1] = s >= 64 ? 0 : w[1] >> s;
+        v = __builtin_bit_cast(bxi4, w);
+    }
+    return v;
 }
 
 // four consecutive elements of one row, of which n exist.  Results are rounded once to T (nearest, ties to even).

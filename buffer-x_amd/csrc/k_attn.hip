@@ -350,7 +350,7 @@ template <> struct Halves<float> { using type = bx_bf16; };
 // elements [k, k + 8) of a row of n floats
 __device__ __forceinline__ void load8(const float* __restrict__ row, int k, int n, float* e)
 {
-    const bxi4 a = bx_load_chunk<float, false>(row, k, n), b = bx_load_chunk<float, false>(row, k + 4, n);
+    const bxi4 a = bx_load_chunk<float>(row, k, n), b = bx_load_chunk<float>(row, k + 4, n);
     __builtin_memcpy(e, &a, 16);
     __builtin_memcpy(e + 4, &b, 16);
 }
@@ -358,7 +358,7 @@ __device__ __forceinline__ void load8(const float* __restrict__ row, int k, int 
 constexpr int waves_of(int bytes, int DP, bool direct)
 {
     if (bytes == 4) return DP == 32 ? 3 : DP == 64 ? 2 : 1;
-    return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (direct ? 0 : 1);             // without spills in the loop
+    return DP == 128 ? 2 : (DP == 32 ? 4 : 3) - (direct ? 0 : 1);            // without spills in the loop
 }
 template <class T, int DP, int NW, bool DIRECT>
 __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn_kernel(AttnK p)
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
                 float e[8];
                 load8(qr, (2 * c + h) * CH, p.D, e);
                 bx_planes(e, w.fq[0][c], w.fq[1][c], w.fq[2][c]);
-            } else w.fq[0][c] = bx_load_chunk<T, DIRECT>(qr, (2 * c + h) * CH, p.D);
+            } else w.fq[0][c] = bx_load_chunk<T>(qr, (2 * c + h) * CH, p.D);
         }
     }
     const float slack = 8.0f / p.c;
@@ -511,18 +511,23 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
         bxi4 rk[LD][RW], rv[LD][RW];
         const auto fetch = [&](int t) {
             const int j0 = base_of(t);
+            const auto rows = [&](const auto& load) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < LD; ++i) {
-                const int e = tid + i * NT, key = j0 + e / CPR, d = e % CPR * CH;
+                for (int i = 0; i < LD; ++i) {
+                    const int e = tid + i * NT, key = j0 + e / CPR, d = e % CPR * CH;
 #pragma unroll
-                for (int j = 0; j < RW; ++j) {
-                    rk[i][j] = rv[i][j] = (bxi4){0, 0, 0, 0};
-                    if (key < sp.kl) {
-                        rk[i][j] = bx_load_chunk<T, false>(kb + (long long)key * p.k_st, d + j * BxElem<T>::CH, p.D);
-                        rv[i][j] = bx_load_chunk<T, false>(vb + (long long)key * p.v_st, d + j * BxElem<T>::CH, p.D);
+                    for (int j = 0; j < RW; ++j) {
+                        rk[i][j] = rv[i][j] = (bxi4){0, 0, 0, 0};
+                        if (key < sp.kl) {
+                            rk[i][j] = load(kb + (long long)key * p.k_st, d + j * BxElem<T>::CH);
+                            rv[i][j] = load(vb + (long long)key * p.v_st, d + j * BxElem<T>::CH);
+                        }
                     }
                 }
-            }
+            };
+            if (p.D == DP) rows([&](const T* row, int k) { return bx_load_whole<T>(row, k); });
+            else if (p.D % BxElem<T>::CH == 0) rows([&](const T* row, int k) { return k < p.D ? bx_load_whole<T>(row, k) : (bxi4){0, 0, 0, 0}; });
+            else rows([&](const T* row, int k) { return bx_load_chunk<T>(row, k, p.D); });
         };
         const auto put = [&](bxi4* to, const bxi4* r) {
             if constexpr (F32) {
@@ -620,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
     {
         const T* qr = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
 #pragma unroll
-        for (int c = 0; c < CPR / 2; ++c) w.fq[0][c] = bx_load_chunk<T, false>(qr, (2 * c + h) * CH, p.D);
+        for (int c = 0; c < CPR / 2; ++c) w.fq[0][c] = bx_load_chunk<T>(qr, (2 * c + h) * CH, p.D);
     }
     const float slack = 8.0f / p.c;
     if (p.D < DP) {
@@ -635,7 +640,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
         for (int k2 = 0; k2 < 2; ++k2) {
             const T* kr = kb + (long long)min(j0 + 32 * k2 + lr, sp.kl - 1) * p.k_st;
 #pragma unroll
-            for (int c = 0; c < CPR / 2; ++c) fk[k2][c] = bx_load_chunk<T, true>(kr, (2 * c + h) * CH, p.D);
+            for (int c = 0; c < CPR / 2; ++c) fk[k2][c] = bx_load_chunk<T>(kr, (2 * c + h) * CH, p.D);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the last tile's V has been read
 #pragma unroll
@@ -778,7 +783,8 @@ Shape shape_of(int n_cu, const bx_attention_args& a)
     Shape s;
     s.DP = padded(a.D);
     const long long R = (long long)a.Lq * (a.Hq / a.Hk);
-    s.rows = R <= 32 && direct_of(a);
+    const bool few = R <= 32;                                // (the number of splits goes by the sizes alone: a workspace fits any alignment)
+    s.rows = few && direct_of(a);
     s.tiles_r = (int)((R + 32 * group_of(a.dtype == BX_TYPE_F32 ? 4 : 2, s.DP) - 1) / (32 * group_of(a.dtype == BX_TYPE_F32 ? 4 : 2, s.DP)));
     const long long base = (long long)s.tiles_r * a.Hk * a.B;
     long long keys = a.Lk;
@@ -787,10 +793,15 @@ Shape shape_of(int n_cu, const bx_attention_args& a)
         keys = span < keys ? span : keys;
     }
     const long long tiles = (keys + BN - 1) / BN;
-    // Rows alone fill the card when there are two workgroups a compute unit; with fewer the keys are split, as long as a part keeps four
-    // tiles of 64 keys (one per wave, or enough that joining does not cost more than it saves).
-    long long n = base > 0 ? 2LL * n_cu / base : 1;
-    if (n > (tiles + 3) / 4) n = (tiles + 3) / 4;
+    // Rows alone fill the card when every slot for a workgroup (by the waves that fit a SIMD) has one -- three where the mask is a triangle,
+    // whose workgroups are of all lengths; with fewer the keys are split, as long as a part keeps eight tiles of 64 keys (four for up to
+    // 32 rows, one per wave): below that joining costs more than it saves.
+    const int bytes = a.dtype == BX_TYPE_F32 ? 4 : 2;
+    const long long slots = (long long)n_cu * (few ? 2 : waves_of(bytes, s.DP, true) * 4 / group_of(bytes, s.DP));
+    const long long want = a.left < 0 && a.right >= 0 && !few ? 3 * slots : slots;
+    const int least = few ? 4 : 8;
+    long long n = base > 0 ? want / base : 1;
+    if (n > (tiles + least - 1) / least) n = (tiles + least - 1) / least;
     if (n > 128) n = 128;
     // A few workgroups a compute unit, unevenly: two halves even them out (two clouds of 5000 keypoints f32, 640 workgroups: 352 -> 323 us).
     if (n <= 1 && base < 4LL * n_cu && tiles >= 32) {

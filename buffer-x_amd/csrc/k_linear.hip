@@ -143,17 +143,19 @@ __device__ __forceinline__ void put_rows(const LinearK& p, bxf16 (&acc)[TN][TM],
 //
 // KS > 1: so many groups of waves take the slices of K in turn, each with its own buffers, and meet in LDS at the end -- for outputs that are
 // too few to fill the card with tiles, where a workgroup's time is that of its loads one after the other.
-template <class T, int BM, int BN, int WGM, int WGN, int KS, bool DIRECT>
+//
+// ONE: sums of a single slice need one buffer, and more workgroups fit a compute unit.
+template <class T, int BM, int BN, int WGM, int WGN, int KS, bool DIRECT, bool ONE>
 __global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(LinearK p)
 {
     constexpr int CH = BxElem<T>::CH, BK = 8 * CH, NW = WGM * WGN, NT = NW * 64;
     constexpr int TM = BM / WGM / 32, TN = BN / WGN / 32;
     constexpr int LX = BM * 8 / NT, LW = BN * 8 / NT;
     static_assert(NT % 128 == 0, "a thread's rows are a multiple of 16 apart: its chunks keep their place in a row");
-    constexpr int PUT = NW * 32 * (TN * 32 + 4) / 4, SLICES = 2 * (BM + BN) * 8;
+    constexpr int PUT = NW * 32 * (TN * 32 + 4) / 4, SLICES = (ONE ? 1 : 2) * (BM + BN) * 8;
     __shared__ bxi4 lds[PUT > KS * SLICES ? PUT : KS * SLICES];
     const int group = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
-    bxi4 *const sx0 = lds + group * SLICES, *const sw0 = sx0 + BM * 8, *const sx1 = sw0 + BN * 8, *const sw1 = sx1 + BM * 8;
+    bxi4 *const sx0 = lds + group * SLICES, *const sw0 = sx0 + BM * 8, *const sx1 = ONE ? sx0 : sw0 + BN * 8, *const sw1 = ONE ? sw0 : sx1 + BM * 8;
     const int tid = threadIdx.x % NT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // tiles in groups of 8 rows of tiles, down the rows first: the tiles that an XCD works on at a time share rows of x and of W
     const int id = (int)bx_xcd_order<32>(blockIdx.x, gridDim.x), gsize = 8 * p.tiles_n, first = id / gsize * 8, gm = min(8, p.tiles_m - first);
@@ -176,9 +178,10 @@ __global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(Linear
     const int wm = (wave / WGN) * TM * 32, wn = (wave % WGN) * TN * 32, lr = lane & 31, h = lane >> 5;
     // LDS addresses: the swizzle is an XOR of address bits below a row
     const int x_at = (wm + lr) * 128 + ((h ^ (lr >> 1 & 7)) * 16), w_at = (wn + lr) * 128 + ((h ^ (lr >> 1 & 7)) * 16);
-    const auto multiply = [&](const bxi4* sx, const bxi4* sw) __attribute__((always_inline)) {
+    const auto multiply = [&](const bxi4* sx, const bxi4* sw, int pairs) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            if (c >= pairs) break;
             bxi4 fx[TM], fw[TN];
 #pragma unroll
             for (int b = 0; b < TM; ++b) fx[b] = *(const bxi4*)((const char*)sx + (x_at ^ (c * 32)) + b * 32 * 128);
@@ -194,16 +197,20 @@ __global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(Linear
     // a slice through registers
     bxi4 rx[LX], rw[LW];
     const auto fetch = [&](int k0) {
+        const auto rows = [&](const auto& load) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < LX; ++i) {
-            const int e = tid + i * NT;
-            rx[i] = bx_load_chunk<T, DIRECT>(x + (long long)min(e >> 3, last_m) * p.ldx, k0 + (e & 7) * CH, p.K);
-        }
+            for (int i = 0; i < LX; ++i) {
+                const int e = tid + i * NT;
+                rx[i] = load(x + (long long)min(e >> 3, last_m) * p.ldx, k0 + (e & 7) * CH);
+            }
 #pragma unroll
-        for (int i = 0; i < LW; ++i) {
-            const int e = tid + i * NT;
-            rw[i] = bx_load_chunk<T, DIRECT>(w + (long long)min(e >> 3, last_n) * p.ldw, k0 + (e & 7) * CH, p.K);
-        }
+            for (int i = 0; i < LW; ++i) {
+                const int e = tid + i * NT;
+                rw[i] = load(w + (long long)min(e >> 3, last_n) * p.ldw, k0 + (e & 7) * CH);
+            }
+        };
+        if (k0 + BK <= p.K) rows([&](const T* row, int k) { return bx_load_whole<T>(row, k); });
+        else rows([&](const T* row, int k) { return bx_load_chunk<T>(row, k, p.K); });
     };
     const auto stage = [&](bxi4* sx, bxi4* sw) {
 #pragma unroll
@@ -232,14 +239,14 @@ __global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(Linear
             __syncthreads();
             const bool odd = i & 1;
             if (s + KS < whole) load(odd ? sx0 : sx1, odd ? sw0 : sw1, s + KS);
-            if (KS == 1 || s < whole) multiply(odd ? sx1 : sx0, odd ? sw1 : sw0);
+            if (KS == 1 || s < whole) multiply(odd ? sx1 : sx0, odd ? sw1 : sw0, 4);
         }
         if (whole * BK < p.K) {
             if (group == 0) fetch(whole * BK);
             __syncthreads();
             if (group == 0) stage(sx0, sw0);
             __syncthreads();
-            if (group == 0) multiply(sx0, sw0);
+            if (group == 0) multiply(sx0, sw0, (p.K - whole * BK + 2 * CH - 1) / (2 * CH));
         }
     } else {
         const int steps = (p.K + BK - 1) / BK;
@@ -248,7 +255,7 @@ __global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(Linear
             __syncthreads();
             const bool odd = i & 1;
             if (s + KS < steps) fetch((s + KS) * BK);
-            if (KS == 1 || s < steps) multiply(odd ? sx1 : sx0, odd ? sw1 : sw0);
+            if (KS == 1 || s < steps) multiply(odd ? sx1 : sx0, odd ? sw1 : sw0, ONE ? (p.K + 2 * CH - 1) / (2 * CH) : 4);
             if (s + KS < steps) stage(odd ? sx0 : sx1, odd ? sw0 : sw1);
         }
     }
@@ -324,20 +331,24 @@ __global__ __launch_bounds__(WGM * WGN * 64) void linear_planes_kernel(LinearK p
 
     bxi4 rx[LX][2], rw[LW][2];
     const auto fetch = [&](int k0) {
+        const auto rows = [&](const auto& load) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < LX; ++i) {
-            const int e = tid + i * NT;
-            const T* row = x + (long long)min(e >> 2, last_m) * p.ldx;
+            for (int i = 0; i < LX; ++i) {
+                const int e = tid + i * NT;
+                const T* row = x + (long long)min(e >> 2, last_m) * p.ldx;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) rx[i][j] = bx_load_chunk<T, false>(row, k0 + (e & 3) * 8 + j * 4, p.K);
-        }
+                for (int j = 0; j < 2; ++j) rx[i][j] = load(row, k0 + (e & 3) * 8 + j * 4);
+            }
 #pragma unroll
-        for (int i = 0; i < LW; ++i) {
-            const int e = tid + i * NT;
-            const T* row = w + (long long)min(e >> 2, last_n) * p.ldw;
+            for (int i = 0; i < LW; ++i) {
+                const int e = tid + i * NT;
+                const T* row = w + (long long)min(e >> 2, last_n) * p.ldw;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) rw[i][j] = bx_load_chunk<T, false>(row, k0 + (e & 3) * 8 + j * 4, p.K);
-        }
+                for (int j = 0; j < 2; ++j) rw[i][j] = load(row, k0 + (e & 3) * 8 + j * 4);
+            }
+        };
+        if (k0 + BK <= p.K) rows([&](const T* row, int k) { return bx_load_whole<T>(row, k); });
+        else rows([&](const T* row, int k) { return bx_load_chunk<T>(row, k, p.K); });
     };
     const auto put = [&](bxi4* plane, int stride, int e, const bxi4* r) {
         float f[8];
@@ -412,7 +423,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void linear_planes_kernel(LinearK p
 
 // Few rows: one workgroup = 16 columns of y x 16 rows, its NW waves split K and meet in LDS.  Operands go from memory to the matrix
 // units directly: a wave reads 64 bytes of 16 rows of W per step, and W is read once per 16 rows of x.
-template <class T, int NW, bool ALIGNED>
+template <class T, int NW>
 __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(LinearK p)
 {
     constexpr int CH = BxElem<T>::CH, BK = 4 * CH, U = 4;
@@ -432,8 +443,8 @@ __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(LinearK p)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = (s0 + u * NW) * BK + q * CH;
-            fw[u] = bx_load_chunk<T, ALIGNED>(wr, k, p.K);
-            fx[u] = bx_load_chunk<T, ALIGNED>(xr, k, p.K);
+            if ((s0 + u * NW + 1) * BK <= p.K) { fw[u] = bx_load_whole<T>(wr, k); fx[u] = bx_load_whole<T>(xr, k); }
+            else { fw[u] = bx_load_chunk<T>(wr, k, p.K); fx[u] = bx_load_chunk<T>(xr, k, p.K); }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) acc = bx_mma16<T>(fw[u], fx[u], acc);
@@ -461,8 +472,18 @@ int launch_tile(hipStream_t s, LinearK k, bool aligned)
     const long long tiles = (long long)k.tiles_n * k.tiles_m;
     if (bx_grid_check("bx_linear", tiles, KS * WGM * WGN * 64) != BX_OK) return BX_ERR_ARG;
     const long long far = (1LL << 31) / (256 * (long long)sizeof(T));
-    if (aligned && k.ldx < far && k.ldw < far) linear_tile_kernel<T, BM, BN, WGM, WGN, KS, true><<<(unsigned)tiles, KS * WGM * WGN * 64, 0, s>>>(k);
-    else linear_tile_kernel<T, BM, BN, WGM, WGN, KS, false><<<(unsigned)tiles, KS * WGM * WGN * 64, 0, s>>>(k);
+    const bool direct = aligned && k.ldx < far && k.ldw < far;
+    constexpr int threads = KS * WGM * WGN * 64;
+    if constexpr (BM == 64 && KS == 1) {
+        if (k.K <= 8 * BxElem<T>::CH) {
+            if (direct) linear_tile_kernel<T, BM, BN, WGM, WGN, 1, true, true><<<(unsigned)tiles, threads, 0, s>>>(k);
+            else linear_tile_kernel<T, BM, BN, WGM, WGN, 1, false, true><<<(unsigned)tiles, threads, 0, s>>>(k);
+            BX_LAUNCH_CHECK();
+            return BX_OK;
+        }
+    }
+    if (direct) linear_tile_kernel<T, BM, BN, WGM, WGN, KS, true, false><<<(unsigned)tiles, threads, 0, s>>>(k);
+    else linear_tile_kernel<T, BM, BN, WGM, WGN, KS, false, false><<<(unsigned)tiles, threads, 0, s>>>(k);
     BX_LAUNCH_CHECK();
     return BX_OK;
 }
@@ -493,8 +514,7 @@ int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
     if (k.M <= 16 || pieces <= n_cu) {
         if (bx_grid_check("bx_linear", pieces, 512) != BX_OK) return BX_ERR_ARG;
         k.tiles_n = (k.N + 15) / 16;
-        if (aligned) linear_rows_kernel<T, 8, true><<<(unsigned)pieces, 512, 0, s>>>(k);
-        else linear_rows_kernel<T, 8, false><<<(unsigned)pieces, 512, 0, s>>>(k);
+        linear_rows_kernel<T, 8><<<(unsigned)pieces, 512, 0, s>>>(k);
         BX_LAUNCH_CHECK();
         return BX_OK;
     }
@@ -506,9 +526,16 @@ int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
         if (tiles(64, 64) <= n_cu) return launch_tile<T, 64, 64, 2, 2, 2>(s, k, aligned);
     }
     if constexpr (sizeof(T) == 2) {
-        // Large outputs want 256 x 256 (16384 x 4096 by K = 1024 bf16 with gelu: 174 us; 175 by 128 x 128, 192 by 64 x 128).
-        if (tiles(256, 256) >= 2 * n_cu) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
-        if (k.N > 64 && tiles(64, 128) >= 4 * n_cu && k.K >= 256) return launch_tile<T, 64, 128, 2, 2>(s, k, aligned);
+        // Large outputs want 256 x 256 (16384 x 4096 by K = 1024 bf16 with gelu: 174 us; 175 by 128 x 128, 192 by 64 x 128).  Rows that are not
+        // aligned go through registers, which larger tiles save most of: 16384 x 4096 by 1023 165 us (240 by 128 x 128, 366 by 64 x 64),
+        // 8000 x 2000 by 700 36 us (66), 30000 x 500 by 501 30 us (37, 56); 100000 x 300 by 65 36 us by 128 x 128 (43, 40 by 64 x 64).
+        if (aligned) {
+            if (tiles(256, 256) >= 2 * n_cu) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
+            if (k.N > 64 && tiles(64, 128) >= 4 * n_cu && k.K >= 256) return launch_tile<T, 64, 128, 2, 2>(s, k, aligned);
+        } else {
+            if (tiles(256, 256) >= n_cu - n_cu / 8 && k.K >= 192) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
+            if (tiles(128, 128) >= n_cu - n_cu / 4) return launch_tile<T, 128, 128, 4, 2>(s, k, aligned);
+        }
     } else if (k.K >= 128) {
         // f32 by planes: 8192 x 4096 by 1024 361 us (442 by 64 x 128, 532 on the f32 units), 10000 x 1024 by 1024 150 us (177), 10000 x 256 by
         // 256 20.4 us (23.3).  Shorter sums are bound by memory either way (700000 x 64 by 32: 62 us both).
@@ -516,6 +543,7 @@ int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
         if (k.N > 64 && tiles(64, 128) >= 4 * n_cu) return launch_planes<64, 128, 2, 2>(s, k);
         return launch_planes<64, 64, 2, 2>(s, k);
     }
+    if (k.N <= 32 && k.K <= 8 * BxElem<T>::CH) return launch_tile<T, 64, 32, 2, 1>(s, k, aligned);
     return launch_tile<T, 64, 64, 2, 2>(s, k, aligned);
 }
 

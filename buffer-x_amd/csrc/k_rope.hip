@@ -49,7 +49,9 @@ template <class T, int N, bool VEC> __device__ __forceinline__ bxi4 load_piece(c
     bxi4 r = {0, 0, 0, 0};
     if constexpr (VEC) {
         if (n > 0) r = *reinterpret_cast<const bxi4*>(p);
-    } else {
+    } else if (n >= N) {
+        r = reinterpret_cast<const BxAny16*>(p)->v;
+    } else if (n > 0) {
         T e[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) e[j] = j < n ? p[j] : (T)0.0f;
@@ -73,6 +75,10 @@ template <class T, int N, bool VEC> __device__ __forceinline__ void store_piece(
         bxi4 r;
         __builtin_memcpy(&r, e, 16);
         if (n > 0) *reinterpret_cast<bxi4*>(p) = r;
+    } else if (n >= N) {
+        bxi4 r;
+        __builtin_memcpy(&r, e, 16);
+        reinterpret_cast<BxAny16*>(p)->v = r;
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j)

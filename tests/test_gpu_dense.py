@@ -123,7 +123,8 @@ def test_linear_few_tiles(ctx, dt, pad, M, N, K):
     _linear_case(ctx, dt, M, N, K, act="silu", pads=(pad, pad, 0, 0))
 
 
-@pytest.mark.parametrize("dt,M,N,K", [("f32", 8200, 1100, 264), ("bf16", 8230, 1030, 256), ("bf16", 33000, 1100, 72), ("f16", 33000, 1027, 100)])
+@pytest.mark.parametrize("dt,M,N,K", [("f32", 8200, 1100, 264), ("bf16", 8230, 1030, 256), ("bf16", 33000, 1100, 72), ("f16", 33000, 1027, 100), ("f16", 33000, 1027, 203),
+                                       ("bf16", 9000, 700, 203)])
 @pytest.mark.parametrize("act", ["none", "gelu"])
 def test_linear_many_tiles(ctx, dt, M, N, K, act):
     _linear_case(ctx, dt, M, N, K, act=act, residual=act == "none")
