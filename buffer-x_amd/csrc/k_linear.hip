@@ -474,7 +474,7 @@ int launch_tile(hipStream_t s, LinearK k, bool aligned)
     const long long far = (1LL << 31) / (256 * (long long)sizeof(T));
     const bool direct = aligned && k.ldx < far && k.ldw < far;
     constexpr int threads = KS * WGM * WGN * 64;
-    if constexpr (BM == 64 && KS == 1) {
+    if constexpr (KS == 1 && BN <= 64) {
         if (k.K <= 8 * BxElem<T>::CH) {
             if (direct) linear_tile_kernel<T, BM, BN, WGM, WGN, 1, true, true><<<(unsigned)tiles, threads, 0, s>>>(k);
             else linear_tile_kernel<T, BM, BN, WGM, WGN, 1, false, true><<<(unsigned)tiles, threads, 0, s>>>(k);
@@ -525,25 +525,26 @@ int linear_of(hipStream_t s, int n_cu, const bx_linear_args& a)
         if (tiles(64, 32) <= n_cu) return launch_tile<T, 64, 32, 2, 1, 4>(s, k, aligned);
         if (tiles(64, 64) <= n_cu) return launch_tile<T, 64, 64, 2, 2, 2>(s, k, aligned);
     }
+    // Up to 32 columns leave half of the other tiles empty: 587689 x 32 by 16 f16 15 us (21 by 64 x 64).
+    if (k.N <= 32) return launch_tile<T, 128, 32, 4, 1>(s, k, aligned);
     if constexpr (sizeof(T) == 2) {
         // Large outputs want 256 x 256 (16384 x 4096 by K = 1024 bf16 with gelu: 174 us; 175 by 128 x 128, 192 by 64 x 128).  Rows that are not
         // aligned go through registers, which larger tiles save most of: 16384 x 4096 by 1023 165 us (240 by 128 x 128, 366 by 64 x 64),
         // 8000 x 2000 by 700 36 us (66), 30000 x 500 by 501 30 us (37, 56); 100000 x 300 by 65 36 us by 128 x 128 (43, 40 by 64 x 64).
         if (aligned) {
-            if (tiles(256, 256) >= 2 * n_cu) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
+            if (k.N > 128 && tiles(256, 256) >= 2 * n_cu) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
             if (k.N > 64 && tiles(64, 128) >= 4 * n_cu && k.K >= 256) return launch_tile<T, 64, 128, 2, 2>(s, k, aligned);
         } else {
-            if (tiles(256, 256) >= n_cu - n_cu / 8 && k.K >= 192) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
-            if (tiles(128, 128) >= n_cu - n_cu / 4) return launch_tile<T, 128, 128, 4, 2>(s, k, aligned);
+            if (k.N > 128 && tiles(256, 256) >= n_cu - n_cu / 8 && k.K >= 192) return launch_tile<T, 256, 256, 4, 4>(s, k, aligned);
+            if (k.N > 64 && tiles(128, 128) >= n_cu - n_cu / 4) return launch_tile<T, 128, 128, 4, 2>(s, k, aligned);
         }
     } else if (k.K >= 128) {
         // f32 by planes: 8192 x 4096 by 1024 361 us (442 by 64 x 128, 532 on the f32 units), 10000 x 1024 by 1024 150 us (177), 10000 x 256 by
         // 256 20.4 us (23.3).  Shorter sums are bound by memory either way (700000 x 64 by 32: 62 us both).
-        if (tiles(128, 256) >= 3 * n_cu) return launch_planes<128, 256, 2, 4>(s, k);
+        if (k.N > 128 && tiles(128, 256) >= 3 * n_cu) return launch_planes<128, 256, 2, 4>(s, k);
         if (k.N > 64 && tiles(64, 128) >= 4 * n_cu) return launch_planes<64, 128, 2, 2>(s, k);
         return launch_planes<64, 64, 2, 2>(s, k);
     }
-    if (k.N <= 32 && k.K <= 8 * BxElem<T>::CH) return launch_tile<T, 64, 32, 2, 1>(s, k, aligned);
     return launch_tile<T, 64, 64, 2, 2>(s, k, aligned);
 }
 

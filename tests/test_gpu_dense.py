@@ -124,7 +124,8 @@ def test_linear_few_tiles(ctx, dt, pad, M, N, K):
 
 
 @pytest.mark.parametrize("dt,M,N,K", [("f32", 8200, 1100, 264), ("bf16", 8230, 1030, 256), ("bf16", 33000, 1100, 72), ("f16", 33000, 1027, 100), ("f16", 33000, 1027, 203),
-                                       ("bf16", 9000, 700, 203)])
+                                       ("bf16", 9000, 700, 203), ("f16", 40000, 30, 200), ("f32", 40000, 17, 9), ("bf16", 140000, 64, 16),
+                                       ("f32", 70000, 64, 136)])
 @pytest.mark.parametrize("act", ["none", "gelu"])
 def test_linear_many_tiles(ctx, dt, M, N, K, act):
     _linear_case(ctx, dt, M, N, K, act=act, residual=act == "none")
