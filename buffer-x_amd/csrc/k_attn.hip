@@ -292,13 +292,15 @@ struct Rows {
     }
 };
 
-// The 32 rows from w0 on over the key tiles [t0, t1), one row after the other by the whole wave, touching nothing but what a row sees: the
-// way of waves that met an infinity or NaN at the edge of a mask.  Lanes are keys for the scores and dimensions for the sums.
+// The rows [r0, r1) over the key tiles [t0, t1), one row after the other by the whole wave, in plain f32 and touching nothing but what a row sees:
+// the way of waves that met an infinity or NaN at the edge of a mask, and of few rows over few keys (attn_short_kernel).  Lanes are keys for the
+// scores and dimensions for the sums.
 template <class T>
-__device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const T* kb, const T* vb, int b, int hk, int w0, int lane, int t0, int t1,
+__device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const T* kb, const T* vb, int b, int hk, int r0, int r1, int lane, int t0, int t1,
                                            int DP, long long part, long long rows)
 {
-    for (int r = w0; r < min(w0 + 32, sp.R); ++r) {
+    constexpr int CH = BxElem<T>::CH;
+    for (int r = r0; r < min(r1, sp.R); ++r) {
         const int qi = r / p.G, qg = r - qi * p.G;
         const int hi = p.right < 0 ? sp.kl : min(sp.kl, qi + sp.off + p.right + 1), lo = p.left < 0 ? 0 : qi + sp.off - p.left;
         const T* q = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
@@ -306,9 +308,21 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
         for (int t = t0; t < t1; ++t) {
             const int j0 = (t < sp.t_sink ? t : sp.t_lo + t - sp.t_sink) * BN, j = j0 + lane;
             const bool see = j < hi && (j >= lo || j < p.sinks);
+            const unsigned long long seen = __ballot(see);
+            if (!seen) continue;
+            const T* k = kb + (long long)min(j, sp.kl - 1) * p.k_st;
             float s = 0.0f;
-            if (see)
-                for (int d = 0; d < p.D; ++d) s = fmaf((float)q[d], (float)kb[(long long)j * p.k_st + d], s);
+            int d = 0;
+#pragma unroll 4
+            for (; d + CH <= p.D; d += CH) {
+                T x[CH], y[CH];
+                const bxi4 cx = bx_load_whole<T>(q, d), cy = bx_load_whole<T>(k, d);
+                __builtin_memcpy(x, &cx, 16);
+                __builtin_memcpy(y, &cy, 16);
+#pragma unroll
+                for (int i = 0; i < CH; ++i) s = fmaf((float)x[i], (float)y[i], s);
+            }
+            for (; d < p.D; ++d) s = fmaf((float)q[d], (float)k[d], s);
             float mx = see ? s : -INFINITY;
 #pragma unroll
             for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
@@ -318,14 +332,21 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
             m = mx;
             l = fmaf(l, alpha, bx_wave_sum(w));
             o0 *= alpha; o1 *= alpha;
-            unsigned long long seen = __ballot(see);
-            while (seen) {
-                const int x = __builtin_ctzll(seen);
-                seen &= seen - 1;
-                const float wx = __shfl(w, x, 64);
-                const T* v = vb + (long long)(j0 + x) * p.v_st;
-                if (lane < p.D) o0 = fmaf(wx, (float)v[lane], o0);
-                if (lane + 64 < p.D) o1 = fmaf(wx, (float)v[lane + 64], o1);
+            for (int x0 = 0; x0 < 64; x0 += 8) {
+                const unsigned some = (unsigned)(seen >> x0) & 255u;
+                if (!some) continue;
+                float v0[8], v1[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const T* v = vb + (long long)min(j0 + x0 + i, sp.kl - 1) * p.v_st;
+                    v0[i] = lane < p.D ? (float)v[lane] : 0.0f;
+                    v1[i] = lane + 64 < p.D ? (float)v[lane + 64] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float wx = __shfl(w, x0 + i, 64);
+                    if (some >> i & 1) { o0 = fmaf(wx, v0[i], o0); o1 = fmaf(wx, v1[i], o1); }
+                }
             }
         }
         if (p.nsplit > 1) {
@@ -343,7 +364,23 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
     }
 }
 
-// DIRECT: 16-byte aligned rows and whole chunks go from memory straight into LDS, two buffers deep; others through registers.
+// Few f32 rows over a tile of keys: a wave per row.  The matrix instructions would multiply 32 rows of 64 keys whatever is there, in 14 000
+// cycles: 773 x 4 x 3 rows of 128 over one key 220 -> 25 us, 4 x 3 rows of 128 over 38 keys 20 -> 9 us, 192 x 3 x 18 rows of 128 over 6 keys 56 -> 30
+// us; but 1000 x 32 rows of 32 over 16 keys 16 -> 44 us, hence the rule in shape_of.  (Halves, sixteen times as fast there, lose by it.)
+__global__ __launch_bounds__(256) void attn_short_kernel(AttnK p)
+{
+    using T = float;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int id = blockIdx.x;
+    const int r = id % p.tiles_r * 4 + wave; id /= p.tiles_r;
+    const int hk = id % p.Hk, b = id / p.Hk;
+    const Span sp = span_of(p, b, r, 1);
+    if (r >= sp.R) return;
+    const T* kb = (const T*)p.k + (long long)b * p.k_sb + (long long)hk * p.k_sh;
+    const T* vb = (const T*)p.v + (long long)b * p.v_sb + (long long)hk * p.v_sh;
+    exact_rows<T>(p, sp, kb, vb, b, hk, r, r + 1, lane, 0, sp.t_all, 0, 0, 0);
+}
+
 template <class T> struct Halves { using type = T; };
 template <> struct Halves<float> { using type = bx_bf16; };
 
@@ -560,7 +597,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
 
     const long long rows = (long long)p.B * p.Hk * p.Lq * p.G, part = (long long)split * rows + (long long)(b * p.Hk + hk) * p.Lq * p.G;
     if (w.spoilt()) {
-        exact_rows<T>(p, sp, kb, vb, b, hk, w0, lane, t0, t1, DP, part, rows);
+        exact_rows<T>(p, sp, kb, vb, b, hk, w0, w0 + 32, lane, t0, t1, DP, part, rows);
         return;
     }
     const float l = w.l + other_half(w.l);
@@ -661,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
     }
     const long long rows = (long long)p.B * p.Hk * p.Lq * p.G, part = (long long)split * rows + (long long)(b * p.Hk + hk) * p.Lq * p.G;
     if (__syncthreads_or(w.spoilt())) {
-        if (wave == 0) exact_rows<T>(p, sp, kb, vb, b, hk, 0, lane, t0, t1, DP, part, rows);
+        if (wave == 0) exact_rows<T>(p, sp, kb, vb, b, hk, 0, 32, lane, t0, t1, DP, part, rows);
         return;
     }
     // every wave lays its rows down in its piece of LDS; then four dimensions of a row a thread, the waves in their order
@@ -766,7 +803,7 @@ int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 // over 140 positions, f16: 39 us, 45 by four waves); four share more of the staging of everything else (clouds f32: 324 us, 425 by two).
 constexpr int group_of(int bytes, int DP) { return bytes == 2 && DP == 32 ? 2 : 4; }
 
-struct Shape { int DP, tiles_r, nsplit; bool rows; };
+struct Shape { int DP, tiles_r, nsplit; bool rows, brief; };
 
 // whether rows of 16-byte aligned whole chunks let K and V skip the registers
 bool direct_of(const bx_attention_args& a)
@@ -809,6 +846,8 @@ Shape shape_of(int n_cu, const bx_attention_args& a)
         if (worst(base) - worst(2 * base) > 0.12) n = 2;
     }
     s.nsplit = n < 1 ? 1 : (int)n;
+    s.brief = few && bytes == 4 && tiles <= 1 && R * (16 + a.Lk) <= 4 * s.DP;
+    if (s.brief) { s.nsplit = 1; s.tiles_r = (int)((R + 3) / 4); }
     return s;
 }
 
@@ -819,10 +858,17 @@ int64_t bytes_of(const Shape& s, const bx_attention_args& a)
 }
 
 template <class T, int DP>
-int launch(hipStream_t s, const AttnK& k, bool rows_form, bool direct)
+int launch(hipStream_t s, const AttnK& k, bool brief, bool rows_form, bool direct)
 {
     constexpr int G = group_of(sizeof(T), DP);
     const unsigned grid = (unsigned)((long long)k.tiles_r * k.Hk * k.B * k.nsplit);
+    if constexpr (sizeof(T) == 4) {
+        if (brief) {
+            attn_short_kernel<<<grid, 256, 0, s>>>(k);
+            BX_LAUNCH_CHECK();
+            return BX_OK;
+        }
+    }
     if (rows_form) attn_rows_kernel<T, DP><<<grid, 256, 0, s>>>(k);
     else if constexpr (sizeof(T) == 4) attn_kernel<T, DP, G, false><<<grid, G * 64, 0, s>>>(k);
     else if (direct) attn_kernel<T, DP, G, true><<<grid, G * 64, 0, s>>>(k);
@@ -848,9 +894,9 @@ int attention_of(hipStream_t s, int n_cu, const bx_attention_args& a)
                      a.B, a.Lq, a.Lk, a.Hk, a.Hq / a.Hk, a.D, a.left, a.right, a.sinks, sh.nsplit, sh.tiles_r,
                      (float)((double)a.scale * 1.4426950408889634)};
     const bool direct = direct_of(a);
-    if (sh.DP == 32) return launch<T, 32>(s, k, sh.rows, direct);
-    if (sh.DP == 64) return launch<T, 64>(s, k, sh.rows, direct);
-    return launch<T, 128>(s, k, sh.rows, direct);
+    if (sh.DP == 32) return launch<T, 32>(s, k, sh.brief, sh.rows, direct);
+    if (sh.DP == 64) return launch<T, 64>(s, k, sh.brief, sh.rows, direct);
+    return launch<T, 128>(s, k, sh.brief, sh.rows, direct);
 }
 
 }  // namespace

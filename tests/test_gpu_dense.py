@@ -398,6 +398,14 @@ def test_attention_one_query(ctx, dt, Lk, window, sinks):
     _attention_case(ctx, dt, 2, 1, Lk, 8, 2, 64, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("Lq,Lk,Hq,Hk,D", [(1, 1, 3, 3, 128), (1, 64, 4, 1, 100), (2, 5, 6, 2, 64), (4, 4, 9, 3, 33), (1, 65, 2, 2, 128), (3, 40, 1, 1, 7)])
+@pytest.mark.parametrize("window,sinks,layout", [((-1, 0), 0, "plain"), ((2, 0), 1, "odd"), ((-1, -1), 0, "heads")])
+def test_attention_few_keys(ctx, dt, Lq, Lk, Hq, Hk, D, window, sinks, layout):
+    _attention_case(ctx, dt, 70, Lq, Lk, Hq, Hk, D, window=window, sinks=sinks, layout=layout,
+                    lens=[(1 + b % Lq, (7 * b) % (Lk + 1)) for b in range(70)])
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("window,sinks", [((-1, -1), 0), ((-1, 0), 0), ((30, 5), 2)])
 def test_attention_ragged(ctx, dt, window, sinks):
