@@ -134,6 +134,13 @@ __device__ __forceinline__ void bx_load_lds16(const void* g, void* lds)
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
+// a barrier behind which every wave's loads into LDS have landed
+__device__ __forceinline__ void bx_sync_landed()
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // Workgroups go to the eight XCDs in turn.  This order gives each XCD runs of C neighbours of the logical order instead, whose operands
 // its L2 then reads once; what does not fill whole rounds keeps its place.
 template <unsigned C> __device__ __forceinline__ unsigned bx_xcd_order(unsigned id, unsigned n)

@@ -491,7 +491,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
             // One step: the weights of tile t (the vector unit) while the scores of tile t + 1 are multiplied (the matrix unit), then the sums
             // of tile t.  K runs one tile ahead of V, and both are loaded one step before they are read.
             const auto step = [&](typename R_::Scores& now, typename R_::Scores& next, int t) __attribute__((always_inline)) {
-                __syncthreads();
+                bx_sync_landed();
                 if (t + 2 < t1) load_k(t + 2);
                 load_v(t + 1);
                 typename R_::Weights u;
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
                 w.settle(next, p.c, slack);
             };
             const auto finish = [&](typename R_::Scores& now) __attribute__((always_inline)) {
-                __syncthreads();
+                bx_sync_landed();
                 typename R_::Weights u;
                 w.weights(now, p.c, u);
                 w.add((t1 - 1 - t0) & 1 ? sv1 : sv0, u);
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
             if (t0 < t1) {
                 typename R_::Scores a, b2;
                 load_k(t0);
-                __syncthreads();
+                bx_sync_landed();
                 if (t0 + 1 < t1) load_k(t0 + 1);
                 load_v(t0);
                 score(a, t0);
@@ -530,7 +530,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
             // small heads: the vector unit has most of the work, and waves that do not see a tile leave it out
             if (t0 < t1) { load_k(t0); load_v(t0); }
             for (int t = t0; t < t1; ++t) {
-                __syncthreads();
+                bx_sync_landed();
                 if (t + 1 < t1) { load_k(t + 1); load_v(t + 1); }
                 if (unseen(t)) continue;
                 typename R_::Scores x;

@@ -236,7 +236,7 @@ __global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(Linear
         };
         if (group < whole) load(sx0, sw0, group);
         for (int s = group, i = 0; i < (whole + KS - 1) / KS; s += KS, ++i) {
-            __syncthreads();
+            bx_sync_landed();
             const bool odd = i & 1;
             if (s + KS < whole) load(odd ? sx0 : sx1, odd ? sw0 : sw1, s + KS);
             if (KS == 1 || s < whole) multiply(odd ? sx1 : sx0, odd ? sw1 : sw0, 4);
