@@ -236,19 +236,25 @@ struct Rows {
                 for (int i = 0; i < 16; ++i) o[t][i] *= alpha;
         }
     }
+    // the weights, and their sum: of the rounded ones (halves), so that what a weight lost is missing above and below the line -- the error of a
+    // row whose weight lies on few keys falls away, and two additions are one instruction
     __device__ __forceinline__ void weights(Scores& x, float c, Weights& w)
     {
-        float sum = 0.0f;
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x.s[k2][i] = __builtin_amdgcn_exp2f(fmaf(x.s[k2][i], c, -mb));
-                sum += x.s[k2][i];
-            }
-        l += sum;
+            for (int i = 0; i < 16; ++i) x.s[k2][i] = __builtin_amdgcn_exp2f(fmaf(x.s[k2][i], c, -mb));
+        if constexpr (sizeof(T) == 4 || NP == 3) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum += x.s[k2][i];
+            l += sum;
+        }
         if constexpr (sizeof(T) == 4) { w.s[0] = x.s[0]; w.s[1] = x.s[1]; }
         else {
+            float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 float e[8];
@@ -256,12 +262,19 @@ struct Rows {
                 for (int j = 0; j < 8; ++j) e[j] = x.s[u / 2][8 * (u % 2) + j];
                 if constexpr (NP == 3) bx_planes(e, w.f[0][u], w.f[1][u], w.f[2][u]);
                 else {
-                    T f[8];
+                    typedef T t2 __attribute__((ext_vector_type(2)));
+                    const t2 one = {(T)1.0f, (T)1.0f};
+                    t2 f[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = (T)e[j];
+                    for (int j = 0; j < 4; ++j) {
+                        f[j] = (t2){(T)e[2 * j], (T)e[2 * j + 1]};
+                        if constexpr (__is_same(T, bx_f16)) sum = __builtin_amdgcn_fdot2(f[j], one, sum, false);
+                        else sum = __builtin_amdgcn_fdot2_f32_bf16(f[j], one, sum, false);
+                    }
                     __builtin_memcpy(&w.f[0][u], f, 16);
                 }
             }
+            if constexpr (NP == 1) l += sum;
         }
     }
     __device__ __forceinline__ void add(const bxi4* sv, const Weights& w)
