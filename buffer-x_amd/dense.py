@@ -80,6 +80,7 @@ def _heads(torch, name, t, weight, out, device, dt, T, D):
             raise ValueError(f"{name}_out and {name}_weight need {name}")
         return 0, None, 0, 0, None, None, None, 0, 0
     H = _sized(torch, name, t, 3, "[T, heads, D]")[1]
+    _need(H < 2**31 and D < 2**31, "sizes of 2^31 or more")
     at = _operand(torch, name, t, device, dt, (T, H, D))
     w = None if weight is None else _operand(torch, name + "_weight", weight, device, dt, (D,))
     st, sh, _ = t.stride()
@@ -96,7 +97,7 @@ def qk_norm_rope_args(torch, device, q, k, pos, freqs, sections, norm, eps, q_we
     if pairs not in PAIRS:
         raise ValueError(f"unknown order of pairs {pairs!r} (known: {tuple(PAIRS)})")
     axes = len(sections)
-    _need(1 <= axes <= 4 and min(sections) >= 0, "sections: the rotation pairs of 1 to 4 axes")
+    _need(1 <= axes <= 4 and 0 <= min(sections) and max(sections) < 2**31, "sections: the rotation pairs of 1 to 4 axes")
     first = q if q is not None else k
     T, _, D = _sized(torch, "q (or k, where q is None)", first, 3, "[T, heads, D]")
     dt, code = first.dtype, _type(torch, first)
@@ -115,7 +116,8 @@ def attention_args(torch, device, q, k, v, scale, window, sinks, q_lens, k_lens,
     _, Lk, Hk, _ = _sized(torch, "k", k, 4, "[B, Lk, heads, D]")
     dt, code, big = q.dtype, _type(torch, q), 2**31 - 1
     left, right = window
-    left, right, sinks = max(-1, min(int(left), big)), max(-1, min(int(right), big)), min(int(sinks), big)
+    _need(max(B, Lq, Lk, Hq, Hk, D) <= big, "sizes of 2^31 or more")          # (what the structure's 32 bits would cut off is seen here)
+    left, right, sinks = (max(-1, min(int(n), big)) for n in (left, right, sinks))
     scale = float(scale) if scale is not None else D ** -0.5 if D > 0 else 0.0
     pq = _operand(torch, "q", q, device, dt, (B, Lq, Hq, D))
     pk, pv = _operand(torch, "k", k, device, dt, (B, Lk, Hk, D)), _operand(torch, "v", v, device, dt, (B, Lk, Hk, D))

@@ -187,6 +187,24 @@ def test_attention_tensors():
             bad()
 
 
+def test_sizes_beyond_the_structures():
+    """what 32 bits of the argument structs would cut off: expanded tensors reach such sizes with one element of memory"""
+    from bufferx_amd import dense
+    far = 2**32 + 1
+    attention = lambda q, k, sinks=0: dense.attention_args(torch, CPU, q, k, k, None, (-1, -1), sinks, None, None, _t(1, 1, 1, 8).expand(q.shape))
+    one = _t(1, 1, 1, 8)
+    for q, k in ((one, one.expand(1, far, 1, 8)), (one.expand(1, far, 1, 8), one), (one.expand(far, 1, 1, 8), one.expand(far, 1, 1, 8)), (one.expand(1, 1, far, 8), one)):
+        with pytest.raises(ValueError):
+            attention(q, k)
+    assert attention(one, one, sinks=-2**32)[0].sinks == -1            # which the library refuses
+    assert attention(one, one, sinks=2**32)[0].sinks == 2**31 - 1
+    q = _t(1, 1, 8).expand(1, far, 8)
+    with pytest.raises(ValueError):
+        dense.qk_norm_rope_args(torch, CPU, q, None, torch.zeros(1, 1), torch.ones(4, dtype=torch.float64), (4,), "rms", 1e-6, None, None, "half", q, None, None)
+    with pytest.raises(ValueError):
+        dense.qk_norm_rope_args(torch, CPU, q[:, :1], None, torch.zeros(1, 1), torch.ones(4, dtype=torch.float64), (far,), "rms", 1e-6, None, None, "half", None, None, None)
+
+
 def test_struct_layouts_match_header(lib):
     """ctypes mirrors of the three argument structs: size and the offset of every field, from a C program compiled against the header."""
     import os
