@@ -28,9 +28,13 @@ struct AttnK {
     float c;                         // scale * log2(e): the softmax runs in powers of two
 };
 
-// what one (row tile, batch entry) has to visit
+// What one (row tile, batch entry) has to visit.  Keys that no row sees are skipped: the rows count what is left, the first `sinks` keys and then
+// those from the window's first one on, and key_of is the key that such a count stands for.  So tiles begin where the window begins and the
+// first keys cost no tile of their own (32768 positions, 16 / 4 heads of 128, bf16, causal window of 1024 + 4: 341 -> 329 us; 1500 x 140
+// positions, 2 / 1 heads of 32, f16, 24 keys to either side + 1: 37.2 -> 33.3 us; the same in f32 103 -> 76 us).
 struct Span {
-    int ql, kl, off, R, t_sink, t_lo, t_all;
+    int ql, kl, off, R, sinks, shift, t_all;
+    __device__ __forceinline__ int key_of(int x) const { return x < sinks ? x : x + shift; }
 };
 
 __device__ __forceinline__ Span span_of(const AttnK& p, int b, int r0, int rows)
@@ -44,10 +48,9 @@ __device__ __forceinline__ Span span_of(const AttnK& p, int b, int r0, int rows)
     const int i0 = r0 / p.G, i1 = (min(r0 + rows, s.R) - 1) / p.G;
     const int hi = p.right < 0 ? s.kl : max(0, min(s.kl, i1 + s.off + p.right + 1));
     const int lo = p.left < 0 ? 0 : max(0, i0 + s.off - p.left);
-    const int t_hi = (hi + BN - 1) / BN;
-    s.t_lo = min(lo / BN, t_hi);
-    s.t_sink = min((min(p.sinks, hi) + BN - 1) / BN, s.t_lo);
-    s.t_all = s.t_sink + t_hi - s.t_lo;
+    s.sinks = p.sinks;
+    s.shift = max(0, lo - p.sinks);                          // (> 0: every row sees all of the first keys)
+    s.t_all = (max(0, hi - s.shift) + BN - 1) / BN;
     return s;
 }
 
@@ -315,15 +318,15 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
     constexpr int CH = BxElem<T>::CH;
     for (int r = r0; r < min(r1, sp.R); ++r) {
         const int qi = r / p.G, qg = r - qi * p.G;
-        const int hi = p.right < 0 ? sp.kl : min(sp.kl, qi + sp.off + p.right + 1), lo = p.left < 0 ? 0 : qi + sp.off - p.left;
+        const int hi = (p.right < 0 ? sp.kl : min(sp.kl, qi + sp.off + p.right + 1)) - sp.shift, lo = p.left < 0 ? 0 : qi + sp.off - p.left - sp.shift;
         const T* q = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
         float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
         for (int t = t0; t < t1; ++t) {
-            const int j0 = (t < sp.t_sink ? t : sp.t_lo + t - sp.t_sink) * BN, j = j0 + lane;
+            const int j0 = t * BN, j = j0 + lane;
             const bool see = j < hi && (j >= lo || j < p.sinks);
             const unsigned long long seen = __ballot(see);
             if (!seen) continue;
-            const T* k = kb + (long long)min(j, sp.kl - 1) * p.k_st;
+            const T* k = kb + (long long)min(sp.key_of(j), sp.kl - 1) * p.k_st;
             float s = 0.0f;
             int d = 0;
 #pragma unroll 4
@@ -351,7 +354,7 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
                 float v0[8], v1[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const T* v = vb + (long long)min(j0 + x0 + i, sp.kl - 1) * p.v_st;
+                    const T* v = vb + (long long)min(sp.key_of(j0 + x0 + i), sp.kl - 1) * p.v_st;
                     v0[i] = lane < p.D ? (float)v[lane] : 0.0f;
                     v1[i] = lane + 64 < p.D ? (float)v[lane + 64] : 0.0f;
                 }
@@ -441,8 +444,8 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
     const bool live = r < sp.R, wave_live = w0 < sp.R;
     const int row = live ? r : sp.R - 1, qi = row / p.G, qg = row - qi * p.G;
     const int wi0 = w0 / p.G, wi1 = (min(w0 + 32, sp.R) - 1) / p.G;
-    const auto hi_of = [&](int i) { return p.right < 0 ? sp.kl : min(sp.kl, i + sp.off + p.right + 1); };
-    const auto lo_of = [&](int i) { return p.left < 0 ? 0 : i + sp.off - p.left; };
+    const auto hi_of = [&](int i) { return (p.right < 0 ? sp.kl : min(sp.kl, i + sp.off + p.right + 1)) - sp.shift; };
+    const auto lo_of = [&](int i) { return p.left < 0 ? 0 : i + sp.off - p.left - sp.shift; };
     const int hi = live ? hi_of(qi) : 0, lo = lo_of(qi);
     const int w_hi0 = wave_live ? hi_of(wi0) : 0, w_hi1 = hi_of(wi1), w_lo0 = lo_of(wi0), w_lo1 = lo_of(wi1);
     {
@@ -458,13 +461,12 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
     }
     const float slack = 8.0f / p.c;
 
-    const auto base_of = [&](int t) { return (t < sp.t_sink ? t : sp.t_lo + t - sp.t_sink) * BN; };
     const auto hide = [&](typename R_::Scores& x, int t) __attribute__((always_inline)) {
-        const int j0 = base_of(t);
+        const int j0 = t * BN;
         if (j0 + BN <= w_hi0 && (j0 >= w_lo1 || j0 + BN <= p.sinks)) return;
         w.hide(x, lo - j0 - 4 * h, hi - j0 - 4 * h, p.sinks - j0 - 4 * h, j0 < p.sinks);
     };
-    const auto unseen = [&](int t) { const int j0 = base_of(t); return !wave_live || j0 >= w_hi1 || (j0 + BN <= w_lo0 && j0 >= p.sinks); };
+    const auto unseen = [&](int t) { const int j0 = t * BN; return !wave_live || j0 >= w_hi1 || (j0 + BN <= w_lo0 && j0 >= p.sinks); };
 
     if constexpr (DIRECT) {
         // LDS position e holds chunk (e % CPR) ^ swizzle of key e / CPR.  Keys behind the sequence repeat its last one: no row sees
@@ -483,14 +485,15 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
         const unsigned ks = (unsigned)(p.k_st * sizeof(T)), vs = (unsigned)(p.v_st * sizeof(T));
         const unsigned ko = key0 * ks + ck * (unsigned)sizeof(T), vo = key0 * vs + cv * (unsigned)sizeof(T);
         const auto load = [&](const T* base, long long st, unsigned bytes, unsigned off, int c, bxi4* to, int t) __attribute__((always_inline)) {
-            const int j0 = base_of(t);
-            const char* first = (const char*)(base + (long long)j0 * st);
-            const bool whole = j0 + BN <= sp.kl;
+            const int x0 = t * BN, j0 = sp.key_of(x0);
             if (c < wk) {
+                if (j0 + BN <= sp.kl && sp.key_of(x0 + BN - 1) == j0 + BN - 1) {
+                    const char* first = (const char*)(base + (long long)j0 * st);
 #pragma unroll
-                for (int i = 0; i < LD; ++i) {
-                    const unsigned key = min(key0 + i * STEP, sp.kl - 1 - j0);
-                    bx_load_lds16(first + (whole ? (unsigned)(i * STEP) * bytes + off : key * bytes + c * (unsigned)sizeof(T)), to + (i * NW + wave) * 64);
+                    for (int i = 0; i < LD; ++i) bx_load_lds16(first + ((unsigned)(i * STEP) * bytes + off), to + (i * NW + wave) * 64);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < LD; ++i) bx_load_lds16(base + ((long long)min(sp.key_of(x0 + key0 + i * STEP), sp.kl - 1) * st + c), to + (i * NW + wave) * 64);
                 }
             }
         };
@@ -560,11 +563,11 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
         constexpr int RW = F32 ? 2 : 1;
         bxi4 rk[LD][RW], rv[LD][RW];
         const auto fetch = [&](int t) {
-            const int j0 = base_of(t);
+            const int x0 = t * BN;
             const auto rows = [&](const auto& load) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < LD; ++i) {
-                    const int e = tid + i * NT, key = j0 + e / CPR, d = e % CPR * CH;
+                    const int e = tid + i * NT, key = sp.key_of(x0 + e / CPR), d = e % CPR * CH;
 #pragma unroll
                     for (int j = 0; j < RW; ++j) {
                         rk[i][j] = rv[i][j] = (bxi4){0, 0, 0, 0};
@@ -668,8 +671,8 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
     R_ w;
     w.init(lane);
     const int h = w.h, lr = w.lr, row = min(lr, sp.R - 1), qi = row / p.G, qg = row - qi * p.G;
-    const auto hi_of = [&](int i) { return p.right < 0 ? sp.kl : min(sp.kl, i + sp.off + p.right + 1); };
-    const auto lo_of = [&](int i) { return p.left < 0 ? 0 : i + sp.off - p.left; };
+    const auto hi_of = [&](int i) { return (p.right < 0 ? sp.kl : min(sp.kl, i + sp.off + p.right + 1)) - sp.shift; };
+    const auto lo_of = [&](int i) { return p.left < 0 ? 0 : i + sp.off - p.left - sp.shift; };
     const int hi = lr < sp.R ? hi_of(qi) : 0, lo = lo_of(qi), i1 = (sp.R - 1) / p.G;
     const int w_hi0 = hi_of(0), w_lo1 = lo_of(i1);
     {
@@ -683,12 +686,12 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
         for (int e = lane; e < BN * CPR; e += 64) sv[e] = zero;
     }
     for (int t = t0 + wave; t < t1; t += NW) {
-        const int j0 = (t < sp.t_sink ? t : sp.t_lo + t - sp.t_sink) * BN;
+        const int j0 = t * BN;
         // keys behind the sequence repeat its last one: no row sees them
         bxi4 fk[2][CPR / 2];
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
-            const T* kr = kb + (long long)min(j0 + 32 * k2 + lr, sp.kl - 1) * p.k_st;
+            const T* kr = kb + (long long)min(sp.key_of(j0 + 32 * k2 + lr), sp.kl - 1) * p.k_st;
 #pragma unroll
             for (int c = 0; c < CPR / 2; ++c) fk[k2][c] = bx_load_chunk<T>(kr, (2 * c + h) * CH, p.D);
         }
@@ -696,7 +699,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const int e = i * 64 + lane, key = e / CPR, cv = ((e % CPR) ^ R_::vswz(key)) * CH;
-            const T* vr = vb + (long long)min(j0 + key, sp.kl - 1) * p.v_st + cv;
+            const T* vr = vb + (long long)min(sp.key_of(j0 + key), sp.kl - 1) * p.v_st + cv;
             if (cv < p.D) bx_load_lds16(vr, sv + i * 64);
         }
         const bool masked = !(j0 + BN <= w_hi0 && (j0 >= w_lo1 || j0 + BN <= p.sinks)) || sp.R < 32;
@@ -839,7 +842,7 @@ Shape shape_of(int n_cu, const bx_attention_args& a)
     const long long base = (long long)s.tiles_r * a.Hk * a.B;
     long long keys = a.Lk;
     if (a.left >= 0 && a.right >= 0) {
-        const long long span = (long long)a.left + a.right + 1 + (R < 128 ? a.Lq : 128 / (a.Hq / a.Hk) + 1) + a.sinks + 2 * BN;
+        const long long span = (long long)a.left + a.right + 1 + (R < 128 ? a.Lq : 128 / (a.Hq / a.Hk) + 1) + a.sinks;
         keys = span < keys ? span : keys;
     }
     const long long tiles = (keys + BN - 1) / BN;

@@ -390,6 +390,16 @@ def test_attention_layouts(ctx, dt, layout, D):
     _attention_case(ctx, dt, 2, 150, 150, 4, 2, D, window=(60, 0), sinks=2, layout=layout)
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,layout", [(32, "plain"), (64, "odd"), (128, "heads")])
+@pytest.mark.parametrize("sinks", [1, 63, 64, 65, 130])
+def test_attention_gap_behind_the_first_keys(ctx, dt, D, layout, sinks):
+    """windows that begin one key before, at, one and many keys behind the end of the first keys, for many rows and for one"""
+    for gap in (-1, 0, 1, 100):
+        _attention_case(ctx, dt, 1, 150, 400, 2, 1, D, window=(250 - sinks - gap, 20), sinks=sinks, layout=layout)
+        _attention_case(ctx, dt, 2, 1, 1200, 4, 1, D, window=(1199 - sinks - gap, 0), sinks=sinks, layout=layout, lens=[(1, 1200), (1, 1190)])
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("Lk", [63, 64, 65, 1000, 4096, 9001])
 @pytest.mark.parametrize("window,sinks", [((-1, 0), 0), ((511, 0), 4), ((100, 0), 150)])
