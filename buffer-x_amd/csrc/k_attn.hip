@@ -816,7 +816,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // waves of a workgroup (32 rows each).  Small heads of halves take two: their tiles are short work and rows come in few (1500 patches of 2 heads
-// over 140 positions, f16: 39 us, 45 by four waves); four share more of the staging of everything else (clouds f32: 324 us, 425 by two).
+// over 140 positions, f16, band of 24: 36 us, 38 by four waves, 46 by one); four share more of the staging of everything else (two clouds of 5000 keypoints,
+// f32: 324 us, 425 by two).
 constexpr int group_of(int bytes, int DP) { return bytes == 2 && DP == 32 ? 2 : 4; }
 
 struct Shape { int DP, tiles_r, nsplit; bool rows, brief; };
