@@ -24,14 +24,14 @@ constexpr int BN = 64;               // keys of a tile
 // either side + 1: 32.9 -> 30.2 us; one query over 8192 keys 17.7 -> 17.2).
 struct Div {
     unsigned m;
-    int s, d;
+    int s;
     __device__ __forceinline__ int operator()(int n) const { return (int)((unsigned long long)(unsigned)n * m >> s); }
 };
 Div div_of(int d)
 {
     int l = 0;
     while ((1LL << l) < d) ++l;
-    return {(unsigned)((1ULL << (31 + l)) / (unsigned)d + 1), 31 + l, d};
+    return {(unsigned)((1ULL << (31 + l)) / (unsigned)d + 1), 31 + l};
 }
 
 struct AttnK {
