@@ -154,9 +154,13 @@ struct Rows {
         return *(const float*)((const char*)sv + v_at + t * 128 + (32 * k2 + 8 * (i / 4) + i % 4) * ROW);
     }
 
-    // the weights as second operands: registers of S^T as they are (f32), or rounded to the type of V -- half a step each, as V's own
-    // values carry
-    struct Weights { bxf16 s[sizeof(T) == 4 ? 2 : 1]; bxi4 f[NP][sizeof(T) == 4 ? 1 : 4]; };
+    // the weights as second operands: registers of S^T as they are (f32), or as the sum of two (halves) or three (f32 by planes) numbers of the
+    // operand's type, each the nearest to what the ones before it left.  Two hold 16 bits of bf16 weights and 22 of f16 ones; one alone loses as
+    // much as the result's own rounding does (2-norm against 64 bits 2.28e-3 where rounding the result alone is 1.65e-3: 32768 positions of 16 / 4
+    // heads of 128, bf16, causal window of 1024 + 4).  The second product costs that case 328 -> 443 us, 1500 x 140 positions of 2 / 1 heads of
+    // 32, f16, a band of 49 + 1 32 -> 37 us, one query over 8192 keys 18.2 -> 18.8.
+    static constexpr int WP = NP == 3 ? 3 : 2;
+    struct Weights { bxf16 s[sizeof(T) == 4 ? 2 : 1]; bxi4 f[WP][sizeof(T) == 4 ? 1 : 4]; };
     static constexpr int PLANE = BN * CPR;                   // chunks of a plane of K or V in LDS
 
     static __device__ __forceinline__ bxf16 mma_planes(const bxi4* a, bxi4 b0, bxi4 b1, bxi4 b2, bxf16 acc)
@@ -180,7 +184,11 @@ struct Rows {
         } else {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if constexpr (NP == 1) acc = bx_mma32<T>(vfrag(sv, t, u), w.f[0][u], acc);
+                if constexpr (NP == 1) {
+                    const bxi4 v = vfrag(sv, t, u);
+                    acc = bx_mma32<T>(v, w.f[1][u], acc);
+                    acc = bx_mma32<T>(v, w.f[0][u], acc);
+                }
                 else {
                     bxi4 v[NP];
 #pragma unroll
@@ -256,25 +264,21 @@ struct Rows {
                 for (int i = 0; i < 16; ++i) o[t][i] *= alpha;
         }
     }
-    // the weights, and their sum: of the rounded ones (halves), so that what a weight lost is missing above and below the line -- the error of a
-    // row whose weight lies on few keys falls away, and two additions are one instruction
+    // the weights, and their sum
     __device__ __forceinline__ void weights(Scores& x, float c, Weights& w)
     {
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
             for (int i = 0; i < 16; ++i) x.s[k2][i] = __builtin_amdgcn_exp2f(fmaf(x.s[k2][i], c, -mb));
-        if constexpr (sizeof(T) == 4 || NP == 3) {
-            float sum = 0.0f;
+        float sum = 0.0f;
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2)
+        for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum += x.s[k2][i];
-            l += sum;
-        }
+            for (int i = 0; i < 16; ++i) sum += x.s[k2][i];
+        l += sum;
         if constexpr (sizeof(T) == 4) { w.s[0] = x.s[0]; w.s[1] = x.s[1]; }
         else {
-            float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 float e[8];
@@ -282,19 +286,16 @@ struct Rows {
                 for (int j = 0; j < 8; ++j) e[j] = x.s[u / 2][8 * (u % 2) + j];
                 if constexpr (NP == 3) bx_planes(e, w.f[0][u], w.f[1][u], w.f[2][u]);
                 else {
-                    typedef T t2 __attribute__((ext_vector_type(2)));
-                    const t2 one = {(T)1.0f, (T)1.0f};
-                    t2 f[4];
+                    T hi[8], lo[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        f[j] = (t2){(T)e[2 * j], (T)e[2 * j + 1]};
-                        if constexpr (__is_same(T, bx_f16)) sum = __builtin_amdgcn_fdot2(f[j], one, sum, false);
-                        else sum = __builtin_amdgcn_fdot2_f32_bf16(f[j], one, sum, false);
+                    for (int j = 0; j < 8; ++j) {
+                        hi[j] = (T)e[j];
+                        lo[j] = (T)(e[j] - (float)hi[j]);
                     }
-                    __builtin_memcpy(&w.f[0][u], f, 16);
+                    __builtin_memcpy(&w.f[0][u], hi, 16);
+                    __builtin_memcpy(&w.f[1][u], lo, 16);
                 }
             }
-            if constexpr (NP == 1) l += sum;
         }
     }
     __device__ __forceinline__ void add(const bxi4* sv, const Weights& w)

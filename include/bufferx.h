@@ -371,7 +371,7 @@ int bx_qk_norm_rope(bx_ctx *ctx, void *stream, const bx_qk_norm_rope_args *args)
  * (the last query stands at the last key).  left / right < 0: no bound on that side.  A query that sees no key gets zeros; keys that it
  * does not see do not touch its result, whatever they hold, infinities and NaN included.  scale in [2^-100, 2^100].
  * q_lens / k_lens: device int32 [B], nullable (Lq / Lk).
- * The softmax weights are rounded to the type of v before they are multiplied (f16 / bf16); f32 as in bx_linear.  Rows that meet an
+ * Softmax weights are multiplied with 16 bits (bf16) or 22 (f16), not rounded to the type of v; f32 as in bx_linear.  Rows that meet an
  * infinity or NaN on the edge of their mask (f32: anywhere) are summed one by one: right, but
  * hundreds of times slower, and rounded differently in the last place.
  * workspace: device memory of bx_attention_workspace(ctx, args) bytes (0: none needed; a host function of the sizes alone), aligned to 16 bytes,

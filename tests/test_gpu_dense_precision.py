@@ -1,0 +1,47 @@
+"""What the dense operators promise beyond the general tolerances of test_gpu_dense.py, on the GPU: how many bits weights and planes keep, and
+what does not change a result at all.  u, e and the counts of roundings are those of that file."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_dense import DEV, DT, E, HALF_STEP, TINY, _attention_inputs, _d, _rand, _visible, _within, ctx  # noqa: F401 (ctx: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+# relative error of a softmax weight as it is multiplied: two bf16 (f16) numbers hold it to half a step of half a step
+WEIGHT = {"f32": 0.0, "f16": 2.0 ** -22, "bf16": 2.0 ** -16}
+
+
+def _exact(q, k, v, scale, left, right, sinks, dt):
+    """one batch entry in 64 bits -> (o, tolerance); the weights are not rounded to the type of v"""
+    ql, Hq, D = q.shape
+    kl, Hk = k.shape[0], k.shape[1]
+    o, tol = torch.zeros(ql, Hq, D, dtype=torch.float64), torch.zeros(ql, Hq, D, dtype=torch.float64)
+    see = _visible(ql, kl, left, right, sinks)
+    n = see.sum(1, keepdim=True)
+    for h in range(Hq):
+        Q, K, V = _d(q[:, h]), _d(k[:, h * Hk // Hq]), _d(v[:, h * Hk // Hq])
+        S = torch.where(see, (Q @ K.t()) * scale, -math.inf)
+        ds = torch.where(see, 2 * (D + 8) * E * (Q.abs() @ K.abs().t()) * scale + 4 * E * S.abs(), 0.0).amax(1, keepdim=True)
+        P = torch.softmax(S, 1)
+        o[:, h] = P @ V
+        # (f16: the second number ends at 2^-25, and the weights of a row sum up to 2^7 at least)
+        low = 2.0 ** -32 * (see.double() @ V.abs()) if dt == "f16" else 0.0
+        tol[:, h] = HALF_STEP[dt] * o[:, h].abs() + ((2 * ds + WEIGHT[dt] + 2 * (n + 64) * E) * (P @ V.abs()) + low) * (1 + 2 * HALF_STEP[dt]) + TINY[dt]
+    return o, tol
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("Lq,Lk,Hq,Hk,D,window,layout", [
+    (130, 130, 4, 2, 32, (24, 24), "packed"), (200, 200, 4, 1, 128, (-1, 0), "packed"), (150, 300, 2, 2, 64, (-1, -1), "plain"),
+    (100, 100, 3, 3, 65, (40, 0), "odd"), (1, 300, 8, 2, 64, (-1, 0), "plain"), (3, 5000, 2, 1, 128, (-1, -1), "heads"), (40, 9, 2, 1, 32, (-1, -1), "plain")])
+def test_attention_weights_keep_their_bits(ctx, dt, Lq, Lk, Hq, Hk, D, window, layout):
+    """f16 and bf16 results are off by their own rounding and little more: in 2-norm a tenth of it, element by element the counted roundings"""
+    q, k, v = _attention_inputs(dt, 1, Lq, Lk, Hq, Hk, D, layout)
+    got = ctx.attention(q, k, v, window=window)[0]
+    want, tol = _exact(q[0], k[0], v[0], D ** -0.5, window[0], window[1], 0, dt)
+    _within(got, want, tol, (dt, Lq, Lk, D))
+    rounded = (want.to(DT[dt]).double() - want).norm()
+    assert float((_d(got) - want).norm()) <= 1.1 * float(rounded)
