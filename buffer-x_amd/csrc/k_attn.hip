@@ -242,7 +242,8 @@ struct Rows {
                 for (int i = 0; i < 16; ++i) x.s[k2][i] = (unsigned)(32 * k2 + 8 * (i / 4) + i % 4 - lo) < n ? x.s[k2][i] : -INFINITY;
         }
     }
-    // the rows' reference values follow where the tile's scores are too far above them
+    // the rows' reference values follow where the tile's scores are too far above them -- each row by its own scores, so that its roundings do not
+    // go by keys that only the wave's other rows see
     __device__ __forceinline__ void settle(const Scores& x, float c, float slack)
     {
         float mx = x.s[0][0];
@@ -251,11 +252,12 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x.s[k2][i]);
         mx = fmaxf(mx, other_half(mx));
-        if (__any(mx > thr)) {
-            const float mn = fmaxf(m, mx);
+        const bool up = mx > thr;
+        if (__any(up)) {
+            const float mn = up ? mx : m;
             // a row that has seen nothing yet has no maximum: its powers are 2^-inf = 0 whatever is subtracted
             const float mc = mn == -INFINITY ? 0.0f : mn * c;
-            const float alpha = __builtin_amdgcn_exp2f(fmaf(m, c, -mc));
+            const float alpha = up ? __builtin_amdgcn_exp2f(fmaf(m, c, -mc)) : 1.0f;
             m = mn; mb = mc - BIAS; thr = mn + slack;
             l *= alpha;
 #pragma unroll

@@ -45,3 +45,22 @@ def test_attention_weights_keep_their_bits(ctx, dt, Lq, Lk, Hq, Hk, D, window, l
     _within(got, want, tol, (dt, Lq, Lk, D))
     rounded = (want.to(DT[dt]).double() - want).norm()
     assert float((_d(got) - want).norm()) <= 1.1 * float(rounded)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("Lq,Lk,Hq,Hk,D,at", [(260, 260, 2, 1, 32, 90), (260, 260, 2, 1, 64, 210), (260, 400, 1, 1, 128, 341), (260, 260, 4, 1, 128, 150),
+                                              (8, 900, 4, 1, 64, 896), (3, 9000, 2, 2, 128, 8998), (260, 260, 3, 1, 40, 77)])
+def test_attention_hidden_keys_change_no_bit(ctx, dt, Lq, Lk, Hq, Hk, D, at):
+    """causal rows in front of a key give the same bits whatever finite numbers that key and those behind it hold, also where the rows that
+    share a wave with them do see it and find it far above all others"""
+    q, k, v = _attention_inputs(dt, 1, Lq, Lk, Hq, Hk, D)
+    first = ctx.attention(q, k, v, window=(-1, 0)).clone()
+    front = at - (Lk - Lq)                                   # the first row that sees key `at`
+    assert 0 < front < Lq
+    for scale in (6.0, -40.0):
+        k2, v2 = k.clone(), v.clone()
+        k2[:, at:] = k2[:, at:] * scale
+        v2[:, at:] = 3.0
+        got = ctx.attention(q, k2, v2, window=(-1, 0))
+        assert torch.equal(got[:, :front], first[:, :front]), (scale, int((got[:, :front] != first[:, :front]).sum()))
+        assert not torch.equal(got[:, front:], first[:, front:])
