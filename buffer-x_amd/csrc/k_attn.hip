@@ -10,7 +10,7 @@
 // V's first operand needs keys along the registers: halves are read from LDS with the transposing 8-byte load (lane group of 16 = 4 keys x 16
 // dimensions), floats one by one.
 //
-// Few rows, many keys: the key tiles are dealt to `nsplit` workgroups that leave (O, m, l) in the workspace and a second kernel
+// Few rows, many keys: the key tiles are dealt to `nsplit` workgroups that leave (O, mb, l) in the workspace and a second kernel
 // joins them in a fixed order.
 #include "bx_ops.h"
 
@@ -83,8 +83,10 @@ __device__ __forceinline__ float other_half(float v)
 // The state of a wave's 32 rows and what one tile of 64 keys in LDS does to it.  K rows lie at chunk c ^ kswz(key), V rows at
 // c ^ vswz(key): the lanes of one LDS access then meet different banks.
 //
-// The reference value m of a row is a maximum that may lag: the weights are 2^((s - m) c) and m follows only when a score exceeds it by
-// more than 2^8 would allow -- rows of like scores rescale O once instead of every few tiles.  O and l belong to the same m at all times.
+// The reference value m of a row is a maximum that may lag: the weights are 2^(s c - mb), mb = m c (rounded), and m follows only when a score
+// exceeds it by more than 2^8 would allow -- rows of like scores rescale O once instead of every few tiles.  O and l belong to the same mb at all
+// times: whatever rescales or joins them goes by the difference of two mb, never by m c again, whose rounding is 1e-5 of a weight where scores are
+// in the hundreds.
 //
 // NP = 3 (f32 tiles): every operand is the sum of three bf16 numbers, a = a0 + a1 + a2 (8 + 8 + 8 bits, each the nearest to what is left: all 24 bits
 // are there).  Six of the nine products are multiplied, the smallest first; the three that are left out are below 2^-26 of a b, less
@@ -98,7 +100,7 @@ struct Rows {
     static constexpr float BIAS = __is_same(T, bx_f16) ? 7.0f : 0.0f;
     bxf16 o[ND];
     bxi4 fq[NP][CPR / 2];
-    float m, thr, mb, l;
+    float thr, mb, l;                                        // thr = m + slack (-inf: no score yet)
     bool edge;                                               // of the wave
     int lane, lr, h;
 
@@ -120,7 +122,7 @@ struct Rows {
             const int key = 4 * h + ((lane & 15) >> 2), d = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
             v_at = key * ROW + ((d / 8) ^ vswz(key)) * 16 + (d & 4) * 2;
         }
-        m = thr = -INFINITY;
+        thr = -INFINITY;
         mb = -BIAS;
         l = 0.0f;
         edge = false;
@@ -254,11 +256,10 @@ struct Rows {
         mx = fmaxf(mx, other_half(mx));
         const bool up = mx > thr;
         if (__any(up)) {
-            const float mn = up ? mx : m;
-            // a row that has seen nothing yet has no maximum: its powers are 2^-inf = 0 whatever is subtracted
-            const float mc = mn == -INFINITY ? 0.0f : mn * c;
-            const float alpha = up ? __builtin_amdgcn_exp2f(fmaf(m, c, -mc)) : 1.0f;
-            m = mn; mb = mc - BIAS; thr = mn + slack;
+            const float to = up ? fmaf(mx, c, -BIAS) : mb;
+            const float alpha = !up ? 1.0f : thr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mb - to);
+            thr = up ? mx + slack : thr;
+            mb = to;
             l *= alpha;
 #pragma unroll
             for (int t = 0; t < ND; ++t)
@@ -266,6 +267,8 @@ struct Rows {
                 for (int i = 0; i < 16; ++i) o[t][i] *= alpha;
         }
     }
+    // what a part's O and l are relative to, for joining parts (-inf: they are zero)
+    __device__ __forceinline__ float reference() const { return thr == -INFINITY ? -INFINITY : mb; }
     // the weights, and their sum
     __device__ __forceinline__ void weights(Scores& x, float c, Weights& w)
     {
@@ -340,7 +343,7 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
         const int qi = p.by_G(r), qg = r - qi * p.G;
         const int hi = (p.right < 0 ? sp.kl : min(sp.kl, qi + sp.off + p.right + 1)) - sp.shift, lo = p.left < 0 ? 0 : qi + sp.off - p.left - sp.shift;
         const T* q = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
-        float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+        float m = -INFINITY, mb = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;       // mb: m c (rounded), -inf before the first score
         for (int t = t0; t < t1; ++t) {
             const int j0 = t * BN, j = j0 + lane;
             const bool see = j < hi && (j >= lo || j < p.sinks);
@@ -363,9 +366,11 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
 #pragma unroll
             for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
             mx = fmaxf(m, mx);
-            const float mc = mx == -INFINITY ? 0.0f : mx * p.c, alpha = __builtin_amdgcn_exp2f(fmaf(m, p.c, -mc));
-            const float w = see ? __builtin_amdgcn_exp2f(fmaf(s, p.c, -(mc - Rows<T, 32>::BIAS))) : 0.0f;
-            m = mx;
+            const float to = mx == -INFINITY ? -INFINITY : fmaf(mx, p.c, -Rows<T, 32>::BIAS);
+            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mb - to);
+            // (rows without a score yet: 2^-inf = 0 whatever is subtracted, and a NaN stays one)
+            const float w = see ? __builtin_amdgcn_exp2f(fmaf(s, p.c, mx == -INFINITY ? 0.0f : -to)) : 0.0f;
+            m = mx; mb = to;
             l = fmaf(l, alpha, bx_wave_sum(w));
             o0 *= alpha; o1 *= alpha;
             for (int x0 = 0; x0 < 64; x0 += 8) {
@@ -390,7 +395,7 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
             if (lane < DP) po[lane] = o0;
             if (lane + 64 < DP) po[lane + 64] = o1;
             float* ml = p.ws + (long long)p.nsplit * rows * DP + (part + r) * 2;
-            if (lane == 0) { ml[0] = m; ml[1] = l; }
+            if (lane == 0) { ml[0] = mb; ml[1] = l; }
         } else {
             const float inv = hi <= 0 ? 0.0f : 1.0f / l;
             T* po = (T*)p.o + (long long)b * p.o_sb + (long long)qi * p.o_st + (long long)(hk * p.G + qg) * p.o_sh;
@@ -650,7 +655,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
                 *reinterpret_cast<bxf4*>(po + 32 * t + 8 * g + 4 * h) = (bxf4){w.o[t][4 * g], w.o[t][4 * g + 1], w.o[t][4 * g + 2], w.o[t][4 * g + 3]};
         if (h == 0) {
             float* ml = p.ws + (long long)p.nsplit * rows * DP + (part + r) * 2;
-            ml[0] = w.m; ml[1] = l;
+            ml[0] = w.reference(); ml[1] = l;
         }
         return;
     }
@@ -747,17 +752,17 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
         for (int g = 0; g < 4; ++g)
             *(bxf4*)&so[lr * DP + (32 * t + 8 * g + 4 * h ^ (lr & 7) * 4)] = (bxf4){w.o[t][4 * g], w.o[t][4 * g + 1], w.o[t][4 * g + 2], w.o[t][4 * g + 3]};
     const float l = w.l + other_half(w.l);
-    if (h == 0) { sm[wave][lr] = w.m; sl[wave][lr] = l; }
+    if (h == 0) { sm[wave][lr] = w.reference(); sl[wave][lr] = l; }
     __syncthreads();
     for (int e = tid; e < sp.R * (DP / 4); e += 256) {
         const int r = e / (DP / 4), d = e % (DP / 4) * 4;
         if (d >= p.D && p.nsplit == 1) continue;
         const float m = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-        const float mc = m == -INFINITY ? 0.0f : m * p.c;
+        const float from = m == -INFINITY ? 0.0f : m;
         float l4 = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < NW; ++x) {
-            const float f = __builtin_amdgcn_exp2f(fmaf(sm[x][r], p.c, -mc));
+            const float f = __builtin_amdgcn_exp2f(sm[x][r] - from);
             const bxf4 o = *(const bxf4*)&((const float*)sv_all[x])[r * DP + (d ^ (r & 7) * 4)];
             l4 = fmaf(f, sl[x][r], l4);
 #pragma unroll
@@ -777,7 +782,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
     }
 }
 
-// joins the parts of a row: weights 2^((m_s - m) c).  DP / 4 lanes have four dimensions each; SG groups of them share the splits of a row and add up
+// joins the parts of a row: weights 2^(mb_s - mb).  DP / 4 lanes have four dimensions each; SG groups of them share the splits of a row and add up
 // in their order, so that a single token's many parts are read together instead of one after the other.
 template <class T, int DP, int SG>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
@@ -798,8 +803,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
     float m = -INFINITY, l = 0.0f;
     bxf4 v = {0.f, 0.f, 0.f, 0.f};
     const auto take = [&](float ms, float ls, const bxf4& o) {
-        const float mn = fmaxf(m, ms), mc = mn == -INFINITY ? 0.0f : mn * p.c;
-        const float a = __builtin_amdgcn_exp2f(fmaf(m, p.c, -mc)), w = __builtin_amdgcn_exp2f(fmaf(ms, p.c, -mc));
+        const float mn = fmaxf(m, ms), from = mn == -INFINITY ? 0.0f : mn;
+        const float a = __builtin_amdgcn_exp2f(m - from), w = __builtin_amdgcn_exp2f(ms - from);
         m = mn;
         l = fmaf(l, a, w * ls);
 #pragma unroll

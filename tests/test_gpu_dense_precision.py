@@ -64,3 +64,31 @@ def test_attention_hidden_keys_change_no_bit(ctx, dt, Lq, Lk, Hq, Hk, D, at):
         got = ctx.attention(q, k2, v2, window=(-1, 0))
         assert torch.equal(got[:, :front], first[:, :front]), (scale, int((got[:, :front] != first[:, :front]).sum()))
         assert not torch.equal(got[:, front:], first[:, front:])
+
+
+@pytest.mark.parametrize("Lq,Lk", [(1, 256), (1, 9000), (5, 700), (40, 9000), (40, 300), (200, 300)])
+@pytest.mark.parametrize("D", [32, 128])
+@pytest.mark.parametrize("at", [3.0, 555.0, -1300.0])
+@pytest.mark.parametrize("spoilt", [False, True])
+def test_attention_far_scores_keep_their_weights(ctx, Lq, Lk, D, at, spoilt):
+    """f32 weights do not suffer where scores lie far from zero: one key of every tile counts, with a score that f32 holds exactly, so that all a
+    weight loses is lost in the softmax.  `spoilt`: an infinity has the first tiles summed row by row, beside others that are not.
+    Scores are up to 3 apart: 2^-24 of that by scale * log2(e), three roundings of the difference, 2^-23 by each power (the weight's, and twice in
+    joining, above and below the line), sums of at most 150 terms in groups of up to 64: 3 e + 3 e + 6 * 2 e + (64 + 4) e, at most 90 e."""
+    rng = np.random.default_rng(Lk + D)
+    score = np.full(Lk, at - 2000.0, dtype=np.float32)
+    some = np.arange(5, Lk, 64)
+    score[some] = at + 3.0 * rng.random(len(some))
+    k = torch.zeros(1, Lk, 1, D, device=DEV)
+    k[0, :, 0, 0] = torch.tensor(score)
+    q = torch.zeros(1, Lq, 1, D, device=DEV)
+    q[..., 0] = 1.0
+    v = _rand(rng, (1, Lk, 1, D), "f32").abs() + 1.0
+    if spoilt:
+        v[0, some[0], 0, 7] = math.inf
+    got = _d(ctx.attention(q, k, v, scale=1.0))[0, :, 0]
+    P = torch.softmax(torch.tensor(score[some], dtype=torch.float64), 0)
+    want = P @ _d(v)[0, some, 0]
+    keep = [d for d in range(D) if d != 7]
+    assert float((got[:, keep] / want[keep] - 1).abs().max()) <= 90 * E
+    assert not spoilt or bool((got[:, 7] == math.inf).all())
