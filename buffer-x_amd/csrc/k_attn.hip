@@ -10,13 +10,26 @@
 // V's first operand needs keys along the registers: halves are read from LDS with the transposing 8-byte load (lane group of 16 = 4 keys x 16
 // dimensions), floats one by one.
 //
-// Few rows, many keys: the key tiles are dealt to `nsplit` workgroups that leave (O, mb, l) in the workspace and a second kernel
+// Few rows, many keys: the key tiles are dealt to `nsplit` workgroups that leave (O, m, l) in the workspace and a second kernel
 // joins them in a fixed order.
 #include "bx_ops.h"
 
 namespace {
 
 constexpr int BN = 64;               // keys of a tile
+
+// f16 weights are held times 2^7: with the 2^8 that the reference value may lag they stay below 2^16 and the smallest keep their digits
+template <class T> __host__ __device__ constexpr float bias_of() { return __is_same(T, bx_f16) ? 7.0f : 0.0f; }
+
+// Weights are 2^(s c - mb), mb = m c - bias rounded, so what a row sums is relative to 2^(m c - over), over = m c - mb.  Scores (times scale * log2(e))
+// of 2^22 and more are too steep for that: m c and the lag of m are rounded by whole units of the exponent there, and a weight could pass the range of
+// its type (below, both together add less than half a unit).  Their weights are 2^((s - m) c), over = 0 (exact_rows).
+constexpr float STEEP = 4194304.0f;  // 2^22
+template <class T> __device__ __forceinline__ float over_of(float m, float c)
+{
+    const float mb = fmaf(m, c, -bias_of<T>());
+    return fabsf(mb) < STEEP ? fmaf(m, c, -mb) : 0.0f;
+}
 
 // n / d for 0 <= n < 2^31 by a multiplication: with l the least for which d <= 2^l, m = floor(2^(31 + l) / d) + 1 is less than 2^32, and n times the
 // excess m d - 2^(31 + l) <= d <= 2^l stays below 2^(31 + l), which is what the quotient can bear.  A division takes some twenty
@@ -83,10 +96,9 @@ __device__ __forceinline__ float other_half(float v)
 // The state of a wave's 32 rows and what one tile of 64 keys in LDS does to it.  K rows lie at chunk c ^ kswz(key), V rows at
 // c ^ vswz(key): the lanes of one LDS access then meet different banks.
 //
-// The reference value m of a row is a maximum that may lag: the weights are 2^(s c - mb), mb = m c (rounded), and m follows only when a score
-// exceeds it by more than 2^8 would allow -- rows of like scores rescale O once instead of every few tiles.  O and l belong to the same mb at all
-// times: whatever rescales or joins them goes by the difference of two mb, never by m c again, whose rounding is 1e-5 of a weight where scores are
-// in the hundreds.
+// The reference value m of a row is a maximum that may lag: m follows only when a score exceeds it by more than 2^8 would allow -- rows of like scores
+// rescale O once instead of every few tiles.  O and l belong to the same mb at all times: whatever rescales or joins them takes over_of into
+// account, as m c alone is 1e-5 of a weight away from mb where scores are in the hundreds.
 //
 // NP = 3 (f32 tiles): every operand is the sum of three bf16 numbers, a = a0 + a1 + a2 (8 + 8 + 8 bits, each the nearest to what is left: all 24 bits
 // are there).  Six of the nine products are multiplied, the smallest first; the three that are left out are below 2^-26 of a b, less
@@ -96,11 +108,10 @@ __device__ __forceinline__ float other_half(float v)
 template <class T, int DP, int NP = 1>
 struct Rows {
     static constexpr int CH = BxElem<T>::CH, CPR = DP / CH, ND = DP / 32;
-    // f16 weights are held times 2^7: with the 2^8 above they stay below 2^16 and the smallest keep their digits (O and l alike)
-    static constexpr float BIAS = __is_same(T, bx_f16) ? 7.0f : 0.0f;
+    static constexpr float BIAS = bias_of<T>();
     bxf16 o[ND];
     bxi4 fq[NP][CPR / 2];
-    float thr, mb, l;                                        // thr = m + slack (-inf: no score yet)
+    float m, mb, l;                                          // m: -inf before the first score
     bool edge;                                               // of the wave
     int lane, lr, h;
 
@@ -122,7 +133,7 @@ struct Rows {
             const int key = 4 * h + ((lane & 15) >> 2), d = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
             v_at = key * ROW + ((d / 8) ^ vswz(key)) * 16 + (d & 4) * 2;
         }
-        thr = -INFINITY;
+        m = -INFINITY;
         mb = -BIAS;
         l = 0.0f;
         edge = false;
@@ -254,11 +265,12 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x.s[k2][i]);
         mx = fmaxf(mx, other_half(mx));
-        const bool up = mx > thr;
+        const bool up = mx > m + slack;
         if (__any(up)) {
             const float to = up ? fmaf(mx, c, -BIAS) : mb;
-            const float alpha = !up ? 1.0f : thr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mb - to);
-            thr = up ? mx + slack : thr;
+            if (__any(up && fabsf(to) >= STEEP && fabsf(mx) < INFINITY)) { edge = true; o[0][0] = NAN; }      // (for spoilt)
+            const float alpha = !up ? 1.0f : m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mb - to);
+            m = up ? mx : m;
             mb = to;
             l *= alpha;
 #pragma unroll
@@ -267,8 +279,6 @@ struct Rows {
                 for (int i = 0; i < 16; ++i) o[t][i] *= alpha;
         }
     }
-    // what a part's O and l are relative to, for joining parts (-inf: they are zero)
-    __device__ __forceinline__ float reference() const { return thr == -INFINITY ? -INFINITY : mb; }
     // the weights, and their sum
     __device__ __forceinline__ void weights(Scores& x, float c, Weights& w)
     {
@@ -318,8 +328,8 @@ struct Rows {
             } else o[t] = weigh(sv, w, t, o[t]);
         }
     }
-    // Whether a wave that met the edge of a mask has anything but numbers in O: 0 times an infinity or NaN of a key that a row does not see
-    // would be in it (exact_rows).
+    // Whether a wave's rows have to be summed again (exact_rows): it met the edge of a mask and has anything but numbers in O -- 0 times an infinity
+    // or NaN of a key that a row does not see would be in it --, or its scores were too steep, which has put a NaN there.
     __device__ __forceinline__ bool spoilt() const
     {
         float z = 0.0f;
@@ -332,8 +342,8 @@ struct Rows {
 };
 
 // The rows [r0, r1) over the key tiles [t0, t1), one row after the other by the whole wave, in plain f32 and touching nothing but what a row sees:
-// the way of waves that met an infinity or NaN at the edge of a mask, and of few rows over few keys (attn_short_kernel).  Lanes are keys for the
-// scores and dimensions for the sums.
+// the way of waves that met an infinity or NaN at the edge of a mask or scores of 2^22, and of few rows over few keys (attn_short_kernel).  Lanes are keys
+// for the scores and dimensions for the sums.  The weights are 2^((s - m) c + over).
 template <class T>
 __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const T* kb, const T* vb, int b, int hk, int r0, int r1, int lane, int t0, int t1,
                                            int DP, long long part, long long rows)
@@ -343,7 +353,7 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
         const int qi = p.by_G(r), qg = r - qi * p.G;
         const int hi = (p.right < 0 ? sp.kl : min(sp.kl, qi + sp.off + p.right + 1)) - sp.shift, lo = p.left < 0 ? 0 : qi + sp.off - p.left - sp.shift;
         const T* q = (const T*)p.q + (long long)b * p.q_sb + (long long)qi * p.q_st + (long long)(hk * p.G + qg) * p.q_sh;
-        float m = -INFINITY, mb = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;       // mb: m c (rounded), -inf before the first score
+        float m = -INFINITY, over = 0.0f, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
         for (int t = t0; t < t1; ++t) {
             const int j0 = t * BN, j = j0 + lane;
             const bool see = j < hi && (j >= lo || j < p.sinks);
@@ -366,11 +376,11 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
 #pragma unroll
             for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
             mx = fmaxf(m, mx);
-            const float to = mx == -INFINITY ? -INFINITY : fmaf(mx, p.c, -Rows<T, 32>::BIAS);
-            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mb - to);
+            const float over_to = over_of<T>(mx, p.c);
+            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - mx, p.c, over_to - over));
             // (rows without a score yet: 2^-inf = 0 whatever is subtracted, and a NaN stays one)
-            const float w = see ? __builtin_amdgcn_exp2f(fmaf(s, p.c, mx == -INFINITY ? 0.0f : -to)) : 0.0f;
-            m = mx; mb = to;
+            const float w = see ? __builtin_amdgcn_exp2f(fmaf(mx == -INFINITY ? s : s - mx, p.c, over_to)) : 0.0f;
+            m = mx; over = over_to;
             l = fmaf(l, alpha, bx_wave_sum(w));
             o0 *= alpha; o1 *= alpha;
             for (int x0 = 0; x0 < 64; x0 += 8) {
@@ -395,7 +405,7 @@ __device__ __forceinline__ void exact_rows(const AttnK& p, const Span& sp, const
             if (lane < DP) po[lane] = o0;
             if (lane + 64 < DP) po[lane + 64] = o1;
             float* ml = p.ws + (long long)p.nsplit * rows * DP + (part + r) * 2;
-            if (lane == 0) { ml[0] = mb; ml[1] = l; }
+            if (lane == 0) { ml[0] = m; ml[1] = l; }
         } else {
             const float inv = hi <= 0 ? 0.0f : 1.0f / l;
             T* po = (T*)p.o + (long long)b * p.o_sb + (long long)qi * p.o_st + (long long)(hk * p.G + qg) * p.o_sh;
@@ -655,7 +665,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn
                 *reinterpret_cast<bxf4*>(po + 32 * t + 8 * g + 4 * h) = (bxf4){w.o[t][4 * g], w.o[t][4 * g + 1], w.o[t][4 * g + 2], w.o[t][4 * g + 3]};
         if (h == 0) {
             float* ml = p.ws + (long long)p.nsplit * rows * DP + (part + r) * 2;
-            ml[0] = w.reference(); ml[1] = l;
+            ml[0] = w.m; ml[1] = l;
         }
         return;
     }
@@ -752,17 +762,17 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
         for (int g = 0; g < 4; ++g)
             *(bxf4*)&so[lr * DP + (32 * t + 8 * g + 4 * h ^ (lr & 7) * 4)] = (bxf4){w.o[t][4 * g], w.o[t][4 * g + 1], w.o[t][4 * g + 2], w.o[t][4 * g + 3]};
     const float l = w.l + other_half(w.l);
-    if (h == 0) { sm[wave][lr] = w.reference(); sl[wave][lr] = l; }
+    if (h == 0) { sm[wave][lr] = w.m; sl[wave][lr] = l; }
     __syncthreads();
     for (int e = tid; e < sp.R * (DP / 4); e += 256) {
         const int r = e / (DP / 4), d = e % (DP / 4) * 4;
         if (d >= p.D && p.nsplit == 1) continue;
         const float m = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-        const float from = m == -INFINITY ? 0.0f : m;
+        const float from = m == -INFINITY ? 0.0f : m, over = over_of<T>(m, p.c);
         float l4 = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < NW; ++x) {
-            const float f = __builtin_amdgcn_exp2f(sm[x][r] - from);
+            const float f = __builtin_amdgcn_exp2f(fmaf(sm[x][r] - from, p.c, over - over_of<T>(sm[x][r], p.c)));
             const bxf4 o = *(const bxf4*)&((const float*)sv_all[x])[r * DP + (d ^ (r & 7) * 4)];
             l4 = fmaf(f, sl[x][r], l4);
 #pragma unroll
@@ -782,7 +792,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnK p)
     }
 }
 
-// joins the parts of a row: weights 2^(mb_s - mb).  DP / 4 lanes have four dimensions each; SG groups of them share the splits of a row and add up
+// joins the parts of a row, each relative to its 2^(m c - over).  DP / 4 lanes have four dimensions each; SG groups of them share the splits of a row and add up
 // in their order, so that a single token's many parts are read together instead of one after the other.
 template <class T, int DP, int SG>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
@@ -802,9 +812,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
     // one pass with a running maximum; four parts are on their way at a time
     float m = -INFINITY, l = 0.0f;
     bxf4 v = {0.f, 0.f, 0.f, 0.f};
-    const auto take = [&](float ms, float ls, const bxf4& o) {
+    const auto take = [&](float ms, float over, float ls, const bxf4& o) {
         const float mn = fmaxf(m, ms), from = mn == -INFINITY ? 0.0f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - from), w = __builtin_amdgcn_exp2f(ms - from);
+        const float a = __builtin_amdgcn_exp2f((m - from) * p.c), w = __builtin_amdgcn_exp2f(fmaf(ms - from, p.c, -over));
         m = mn;
         l = fmaf(l, a, w * ls);
 #pragma unroll
@@ -822,7 +832,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (s0 + j * SG < p.nsplit) take(ms[j], ls[j], o[j]);
+                if (s0 + j * SG < p.nsplit) take(ms[j], over_of<T>(ms[j], p.c), ls[j], o[j]);
         }
     }
     if constexpr (SG > 1) {
@@ -831,7 +841,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p)
         __syncthreads();
         if (g > 0) return;
 #pragma unroll
-        for (int j = 1; j < SG; ++j) take(sm[rb][j], sl[rb][j], so[rb][j][x]);
+        for (int j = 1; j < SG; ++j) take(sm[rb][j], 0.0f, sl[rb][j], so[rb][j][x]);
     }
     if (!live || d >= p.D) return;
     const bool empty = p.right >= 0 && qi + kl - ql + p.right + 1 <= 0;

@@ -369,11 +369,12 @@ int bx_qk_norm_rope(bx_ctx *ctx, void *stream, const bx_qk_norm_rope_args *args)
  *   o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys that query i of a batch entry sees:
  *   j < k_len,  j <= p_i + right (right >= 0),  j >= p_i - left (left >= 0) or j < sinks,      p_i = i + k_len - q_len
  * (the last query stands at the last key).  left / right < 0: no bound on that side.  A query that sees no key gets zeros; keys that it
- * does not see do not touch its result, whatever they hold, infinities and NaN included.  scale in [2^-100, 2^100].
+ * does not see do not touch its result, whatever they hold, infinities and NaN included (the last place of it in one case, below).  scale in
+ * [2^-100, 2^100].
  * q_lens / k_lens: device int32 [B], nullable (Lq / Lk).
  * Softmax weights are multiplied with 16 bits (bf16) or 22 (f16), not rounded to the type of v; f32 as in bx_linear.  Rows that meet an
- * infinity or NaN on the edge of their mask (f32: anywhere) are summed one by one: right, but
- * hundreds of times slower, and rounded differently in the last place.
+ * infinity or NaN on the edge of their mask (f32: anywhere), or scores times scale of about 2^21 and more, are summed one by one with the 31 that
+ * share a wave with them: right, but hundreds of times slower, and rounded differently in the last place.
  * workspace: device memory of bx_attention_workspace(ctx, args) bytes (0: none needed; a host function of the sizes alone), aligned to 16 bytes,
  * used until the call has run and by no other call meanwhile; BX_ERR_STATE when it is too small.               */
 typedef struct bx_attention_args {

@@ -92,3 +92,27 @@ def test_attention_far_scores_keep_their_weights(ctx, Lq, Lk, D, at, spoilt):
     keep = [d for d in range(D) if d != 7]
     assert float((got[:, keep] / want[keep] - 1).abs().max()) <= 90 * E
     assert not spoilt or bool((got[:, 7] == math.inf).all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("Lq,Lk", [(1, 200), (1, 9000), (40, 200), (130, 500), (40, 9000)])
+@pytest.mark.parametrize("D", [32, 128])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("steps", [1.0, 90.0])
+def test_attention_steep_scores(ctx, dt, Lq, Lk, D, sign, steps):
+    """scores that f32 holds exactly, 2^30 (f16) or 2^40 away from zero, which times the scale differ by `steps` times a whole number, in
+    units of 2^7 (2^17) before it: the weights go by the differences, which are exact.  The same count of roundings as for far scores, and 2^-23 of
+    a score difference of up to 255 that a power still sees (those of more than 126 have no weight): 90 e + 2 * 126 e."""
+    big, unit = (2.0 ** 15, 2.0 ** 7) if dt == "f16" else (2.0 ** 20, 2.0 ** 17)
+    rng = np.random.default_rng(Lq + Lk + D)
+    j = rng.integers(0, 256, Lk)
+    k = torch.zeros(1, Lk, 1, D, dtype=DT[dt], device=DEV)
+    k[..., 0] = sign * big
+    k[0, :, 0, 1] = torch.tensor(j, dtype=DT[dt])
+    q = torch.zeros(1, Lq, 1, D, dtype=DT[dt], device=DEV)
+    q[..., 0], q[..., 1] = big, unit
+    v = _rand(rng, (1, Lk, 1, D), dt).abs() + 1.0
+    got = _d(ctx.attention(q, k, v, scale=steps / unit))[0, :, 0]
+    want = torch.softmax(torch.tensor(j, dtype=torch.float64) * float(np.float32(steps / unit)) * unit, 0) @ _d(v)[0, :, 0]
+    n = min(Lk, 9000)
+    assert float((got / want - 1).abs().max()) <= HALF_STEP[dt] * (1 + 2 * HALF_STEP[dt]) + WEIGHT[dt] + (90 + 252 + 2 * n / 64) * E
