@@ -18,10 +18,12 @@ namespace {
 
 constexpr int BN = 64;               // keys of a tile
 
-// f16 weights are held times 2^7: with the 2^8 that the reference value may lag they stay below 2^16 and the smallest keep their digits
-template <class T> __host__ __device__ constexpr float bias_of() { return __is_same(T, bx_f16) ? 7.0f : 0.0f; }
+// f16 weights are held times 2^7: with the 2^8 that the reference value may lag they stay below 2^16 and the smallest keep their digits.  bf16
+// weights are held times 2^-8: none is above 1, so that sums over large values pass the range of f32 no sooner than sum p v would with the largest p
+// at 1.  (f32 needs none: sums that are not numbers are formed again by exact_rows, whose weights are at most 1.)
+template <class T> __host__ __device__ constexpr float bias_of() { return __is_same(T, bx_f16) ? 7.0f : __is_same(T, bx_bf16) ? -8.0f : 0.0f; }
 
-// Weights are 2^(s c - mb), mb = m c - bias rounded, so what a row sums is relative to 2^(m c - over), over = m c - mb.  Scores (times scale * log2(e))
+// Weights are 2^(s c - mb), mb = m c - bias rounded, so that what a row sums is relative to 2^(m c - over), over = m c - mb.  Scores (times scale * log2(e))
 // of 2^22 and more are too steep for that: m c and the lag of m are rounded by whole units of the exponent there, and a weight could pass the range of
 // its type (below, both together add less than half a unit).  Their weights are 2^((s - m) c), over = 0 (exact_rows).
 constexpr float STEEP = 4194304.0f;  // 2^22
@@ -108,7 +110,7 @@ __device__ __forceinline__ float other_half(float v)
 template <class T, int DP, int NP = 1>
 struct Rows {
     static constexpr int CH = BxElem<T>::CH, CPR = DP / CH, ND = DP / 32;
-    static constexpr float BIAS = bias_of<T>();
+    static constexpr float BIAS = NP == 3 ? bias_of<float>() : bias_of<T>();
     bxf16 o[ND];
     bxi4 fq[NP][CPR / 2];
     float m, mb, l;                                          // m: -inf before the first score

@@ -116,3 +116,16 @@ def test_attention_steep_scores(ctx, dt, Lq, Lk, D, sign, steps):
     want = torch.softmax(torch.tensor(j, dtype=torch.float64) * float(np.float32(steps / unit)) * unit, 0) @ _d(v)[0, :, 0]
     n = min(Lk, 9000)
     assert float((got / want - 1).abs().max()) <= HALF_STEP[dt] * (1 + 2 * HALF_STEP[dt]) + WEIGHT[dt] + (90 + 252 + 2 * n / 64) * E
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("Lq,Lk,D", [(1, 200, 64), (32, 256, 64), (64, 256, 128), (256, 192, 32), (64, 192, 65), (64, 9024, 128), (130, 190, 32)])
+def test_attention_large_values(ctx, dt, Lq, Lk, D):
+    """values of up to 2^127 / Lk and scores that rise by 5 along the keys: sums of weights of at most 1 times values stay in f32's range"""
+    rng = np.random.default_rng(D)
+    q, k = torch.zeros(1, Lq, 1, D, dtype=DT[dt], device=DEV), torch.zeros(1, Lk, 1, D, dtype=DT[dt], device=DEV)
+    q[..., 0] = 1.0
+    k[0, :, 0, 0] = torch.arange(Lk, device=DEV) * (5.0 / Lk)
+    v = torch.tensor((0.5 + 0.5 * rng.random((1, Lk, 1, D))) * 2.0 ** 127 / Lk, dtype=torch.float32).to(DT[dt]).to(DEV)
+    want, tol = _exact(q[0], k[0], v[0], 1.0, -1, -1, 0, dt)
+    _within(ctx.attention(q, k, v, scale=1.0)[0], want, tol)
