@@ -3,8 +3,11 @@ types, shapes, devices and strides are checked here, overlaps and ranges in the 
 are the calls; nothing here touches the GPU.
 
 Unlike the stage entry points these operators neither convert nor copy what they are given: a tensor of another type, on another
-device or with a strided innermost dimension is refused (ValueError).  They have no backward pass and refuse tensors that ask for one.
+device, with a strided innermost dimension or whose memory does not hold its values is refused (ValueError).  They have no derivatives and
+refuse tensors that ask for one, and they are nothing that a tracer can record.
 """
+import sys
+
 from . import lib
 
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
@@ -27,11 +30,29 @@ def _need(ok, what):
         raise ValueError(what)
 
 
+_STATE = []
+
+
+def _eager(torch):
+    """refuses what would see only the tensors around a call and not the call: a tracer would record an output that nothing writes"""
+    if not _STATE:
+        from torch.autograd import forward_ad
+        _STATE.extend((torch._C._get_tracing_state, forward_ad))
+    if _STATE[0]() is not None:
+        raise ValueError("these operators cannot be traced (torch.jit.trace)")
+    proxy = sys.modules.get("torch.fx.experimental.proxy_tensor")             # (not there: nobody traces with it)
+    if proxy is not None and proxy.get_proxy_mode() is not None:
+        raise ValueError("these operators cannot be traced (make_fx)")
+
+
 def _operand(torch, name, t, device, dtype, shape):
     """the address of `t`, an operand of this type and shape on this device; its innermost dimension has to be contiguous"""
     try:                                                      # the checks below in one go: a call of a few microseconds pays for each
-        if t.dtype is dtype and t.shape == shape and t.device == device and not t.requires_grad and (t.stride(-1) == 1 or shape[-1] <= 1):
-            return t.data_ptr()
+        if (t.dtype is dtype and t.shape == shape and t.device == device and not t.requires_grad and (t.stride(-1) == 1 or shape[-1] <= 1) and
+                not t.is_neg() and _STATE[1]._current_level < 0):
+            at = t.data_ptr()
+            if at:
+                return at
     except AttributeError:
         pass
     if not isinstance(t, torch.Tensor):
@@ -46,7 +67,14 @@ def _operand(torch, name, t, device, dtype, shape):
         raise ValueError(f"{name}: the innermost dimension has to be contiguous")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: these operators have no backward pass (use torch.no_grad() or detach())")
-    return t.data_ptr()
+    if _STATE[1].unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a tangent: these operators have no derivatives")
+    if t.is_neg():
+        raise ValueError(f"{name} is a negated view, whose memory holds other values (use resolve_neg())")
+    at = t.data_ptr()
+    if not at and t.numel():
+        raise ValueError(f"{name} has no memory")
+    return at
 
 
 def _sized(torch, name, t, dims, what):
@@ -56,6 +84,7 @@ def _sized(torch, name, t, dims, what):
 
 
 def linear_args(torch, device, x, weight, bias, act, residual, out, m_dev):
+    _eager(torch)
     M, K = _sized(torch, "x", x, 2, "[M, K]")
     N = _sized(torch, "weight", weight, 2, "[N, K]")[0]
     dt, code = x.dtype, _type(torch, x)
@@ -92,6 +121,7 @@ def _heads(torch, name, t, weight, out, device, dt, T, D):
 
 
 def qk_norm_rope_args(torch, device, q, k, pos, freqs, sections, norm, eps, q_weight, k_weight, pairs, q_out, k_out, m_dev):
+    _eager(torch)
     if norm not in NORMS:
         raise ValueError(f"unknown norm {norm!r} (known: {tuple(NORMS)})")
     if pairs not in PAIRS:
@@ -112,6 +142,7 @@ def qk_norm_rope_args(torch, device, q, k, pos, freqs, sections, norm, eps, q_we
 
 
 def attention_args(torch, device, q, k, v, scale, window, sinks, q_lens, k_lens, out):
+    _eager(torch)
     B, Lq, Hq, D = _sized(torch, "q", q, 4, "[B, Lq, heads, D]")
     _, Lk, Hk, _ = _sized(torch, "k", k, 4, "[B, Lk, heads, D]")
     dt, code, big = q.dtype, _type(torch, q), 2**31 - 1
