@@ -16,13 +16,45 @@ struct RopeK {
     float eps;
 };
 
-// sin and cos of x to binary64 precision for |x| < 2^50: x - n pi/2 in two fused steps, then the series on [-pi/4, pi/4].  Positions
-// times frequencies reach 1e5 rad and more, where a product in f32 has lost the angle.
+// 1 / (2 pi), 1152 bits behind the point: as many turns as the largest binary64 number of radians leaves a fraction of
+__device__ const unsigned long long TURN[18] = {
+    0x28be60db9391054aULL, 0x7f09d5f47d4d3770ULL, 0x36d8a5664f10e410ULL,
+    0x7f9458eaf7aef158ULL, 0x6dc91b8e909374b8ULL, 0x01924bba82746487ULL,
+    0x3f877ac72c4a69cfULL, 0xba208d7d4baed121ULL, 0x3a671c09ad17df90ULL,
+    0x4e64758e60d4ce7dULL, 0x272117e2ef7e4a0eULL, 0xc7fe25fff7816603ULL,
+    0xfbcbc462d6829b47ULL, 0xdb4d9fb3c9f2c26dULL, 0xd3d18fd9a797fa8bULL,
+    0x5d49eeb1faf97c5eULL, 0xcf41ce7de294a4baULL, 0x9afed7ec47e35742ULL};
+
+// |x| >= 2^52 radians: x = m 2^e with whole m < 2^53, e >= 0.  Of the digits of 1 / (2 pi) those above 2^-e make whole turns; m times the next 128 is,
+// modulo 2^128, the fraction of a turn, off by 2^-75 of one.  q = the nearest quarter, r = what is left of it in radians.
+__device__ __forceinline__ double far_angle(double x, int& q)
+{
+    const unsigned long long bits = __builtin_bit_cast(unsigned long long, x) & ~(1ULL << 63);
+    const int e = min((int)(bits >> 52) - 1075, 971), at = e >> 6, sh = e & 63;
+    const unsigned long long m = (bits & ((1ULL << 52) - 1)) | 1ULL << 52;
+    unsigned long long u1 = TURN[at], u0 = TURN[at + 1];
+    if (sh > 0) { u1 = u1 << sh | u0 >> (64 - sh); u0 = u0 << sh | TURN[at + 2] >> (64 - sh); }
+    const unsigned long long f = m * u1 + __umul64hi(m, u0);
+    const unsigned long long n = (f + (1ULL << 61)) >> 62;
+    const double r = (double)(long long)(f - (n << 62)) * (1.57079632679489655800e+00 * 0x1p-62);
+    q = x < 0.0 ? -(int)n : (int)n;
+    // (infinities and NaN have no angle)
+    return bits >= 0x7ffULL << 52 ? x - x : x < 0.0 ? -r : r;
+}
+
+// sin and cos of x: the nearest multiple of pi/2 is taken off in two fused steps (beyond 2^52 by far_angle), then the series on [-pi/4, pi/4].  Their
+// ends are 3e-14 off; the reduction adds 3e-12 at 2^50 and 7e-10 at 2^52, where f32 results keep 6e-8.  Positions times frequencies reach 1e5 rad
+// and more, where a product in f32 has lost the angle.
 __device__ __forceinline__ void sincos64(double x, float& s, float& c)
 {
-    const double n = rint(x * 0.63661977236758134308);
-    double r = fma(-n, 1.57079632679489655800e+00, x);
-    r = fma(-n, 6.12323399573676603587e-17, r);
+    double r;
+    int m;
+    if (fabs(x) < 0x1p52) {
+        const double n = rint(x * 0.63661977236758134308);
+        r = fma(-n, 1.57079632679489655800e+00, x);
+        r = fma(-n, 6.12323399573676603587e-17, r);
+        m = (int)(long long)n;
+    } else r = far_angle(x, m);
     const double z = r * r;
     double a = fma(z, 1.0 / 6227020800.0, -1.0 / 39916800.0);
     a = fma(z, a, 1.0 / 362880.0);
@@ -37,7 +69,6 @@ __device__ __forceinline__ void sincos64(double x, float& s, float& c)
     b = fma(z, b, 1.0 / 24.0);
     b = fma(z, b, -0.5);
     const double cs = fma(z, b, 1.0);
-    const int m = (int)((long long)n & 3);
     const double so = (m & 1) ? cs : sn, co = (m & 1) ? sn : cs;
     s = (float)((m & 2) ? -so : so);
     c = (float)(((m + 1) & 2) ? -co : co);

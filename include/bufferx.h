@@ -340,7 +340,8 @@ int bx_linear(bx_ctx *ctx, void *stream, const bx_linear_args *args);
  *   then rotation pair p of axis a:  (y_i, y_j) -> (y_i cos t - y_j sin t, y_j cos t + y_i sin t),  t = pos[token][a] * freqs[p].
  * sections[a] = number of pairs of axis a (axes 1..4; the pairs of axis 0 come first, P = their sum, 2 P <= D); (i, j) = (p, p + P)
  * with BX_PAIRS_HALF, (2 p, 2 p + 1) with BX_PAIRS_INTERLEAVED; elements from 2 P on are not rotated.
- * pos [T][axes] float32 or int32, freqs float64 [P] (radians per unit of position).  m_dev (nullable): device count of the tokens
+ * pos [T][axes] float32 or int32, freqs float64 [P] (radians per unit of position); t is their binary64 product, of any size (NaN where it
+ * is not finite).  m_dev (nullable): device count of the tokens
  * in use.  q_out may be q itself and k_out k itself (same strides); interleaved rows of one buffer are not an overlap. */
 #define BX_NORM_NONE 0
 #define BX_NORM_RMS 1

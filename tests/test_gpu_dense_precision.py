@@ -129,3 +129,39 @@ def test_attention_large_values(ctx, dt, Lq, Lk, D):
     v = torch.tensor((0.5 + 0.5 * rng.random((1, Lk, 1, D))) * 2.0 ** 127 / Lk, dtype=torch.float32).to(DT[dt]).to(DEV)
     want, tol = _exact(q[0], k[0], v[0], 1.0, -1, -1, 0, dt)
     _within(ctx.attention(q, k, v, scale=1.0)[0], want, tol)
+
+
+@pytest.mark.parametrize("power", [48, 51, 52, 53, 54, 56, 60, 64, 90, 127, 300, 900, 1023])
+@pytest.mark.parametrize("pairs,whole", [("half", False), ("interleaved", True)])
+def test_rope_far_angles(ctx, power, pairs, whole):
+    """angles of up to 2^1024 rad are turned by, not scaled by: sine and cosine of the binary64 product, each off by half a step of f32 (and 7e-10
+    where the product is close to 2^52), three products and a sum: 8 e (|a| + |b|)"""
+    T, D = 40, 24
+    rng = np.random.default_rng(power)
+    x = _rand(rng, (T, 2, D), "f32")
+    p = rng.integers(-2 ** 31 + 1, 2 ** 31 - 1, (T, 1)) | 2 ** 30 if whole else (rng.random((T, 1)) + 1) * rng.choice([-1.0, 1.0], (T, 1))
+    p = torch.tensor(p, dtype=torch.int32 if whole else torch.float32, device=DEV)
+    freqs = torch.tensor((0.5 + 0.5 * rng.random(8)) * 2.0 ** (power - (31 if whole else 1)), dtype=torch.float64, device=DEV)
+    y = _d(ctx.qk_norm_rope(x, None, p, freqs, (8,), norm="none", pairs=pairs)[0])
+    t = (_d(p) * _d(freqs)).numpy()
+    assert np.isfinite(t).all() and np.abs(t).max() >= 2.0 ** (power - 2)
+    cos, sin = (torch.tensor(np.vectorize(f)(t))[:, None] for f in (math.cos, math.sin))
+    X = _d(x)
+    i = torch.arange(8) if pairs == "half" else 2 * torch.arange(8)
+    j = i + 8 if pairs == "half" else i + 1
+    a, b = X[..., i], X[..., j]
+    tol = (8 * E + 1e-9) * (a.abs() + b.abs())
+    assert bool(((y[..., i] - (a * cos - b * sin)).abs() <= tol).all()) and bool(((y[..., j] - (b * cos + a * sin)).abs() <= tol).all())
+    assert torch.equal(y[..., 16:], X[..., 16:])
+
+
+def test_rope_angles_that_are_none(ctx):
+    """an infinite or undefined angle leaves NaN in its pairs and nothing anywhere else"""
+    x = _rand(np.random.default_rng(0), (4, 1, 8), "f32")
+    p = torch.tensor([[1.0], [math.inf], [math.nan], [-3e38]], device=DEV)
+    freqs = torch.tensor([0.0, 1.0, 1e300], dtype=torch.float64, device=DEV)
+    y = ctx.qk_norm_rope(x, None, p, freqs, (3,), norm="none")[0][:, 0]
+    nan = torch.zeros(4, 8, dtype=torch.bool)
+    nan[1, :6] = nan[2, :6] = True                           # (0 * inf too)
+    nan[3, 2] = nan[3, 5] = True                             # 3e38 * 1e300
+    assert torch.equal(torch.isnan(y).cpu(), nan) and torch.equal(y[:, 6:], x[:, 0, 6:])
