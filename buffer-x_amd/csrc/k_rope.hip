@@ -179,10 +179,17 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeK p, int tpb)
             for (int i = 0; i < N; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
 #pragma unroll
             for (int k = LPR / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, LPR);
-            const float l2 = sqrtf(sum);
-            const float f = p.norm == BX_NORM_RMS ? 1.0f / sqrtf(sum / (float)p.D + p.eps) : 1.0f / (l2 < p.eps ? p.eps : l2);
+            // x / d, by a product with 1 / d and what that leaves of x: as a division rounds it.  (A d that is zero or not finite has no such rest: d = 0
+            // there makes it x, which counts for nothing.)
+            const float l2 = sqrtf(sum), d = p.norm == BX_NORM_RMS ? sqrtf(sum / (float)p.D + p.eps) : l2 < p.eps ? p.eps : l2, f = 1.0f / d;
+            const bool safe = d > 0x1p-100f && d < 0x1p100f;
+            const float dr = safe ? d : 0.0f, fr = safe ? f : 0.0f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) { a[i] *= f; b[i] *= f; }
+            for (int i = 0; i < N; ++i) {
+                const float ya = a[i] * f, yb = b[i] * f;
+                a[i] = fmaf(fmaf(-ya, dr, a[i]), fr, ya);
+                b[i] = fmaf(fmaf(-yb, dr, b[i]), fr, yb);
+            }
         }
         if (w) {
             float wa[N], wb[N];

@@ -165,3 +165,19 @@ def test_rope_angles_that_are_none(ctx):
     nan[1, :6] = nan[2, :6] = True                           # (0 * inf too)
     nan[3, 2] = nan[3, 5] = True                             # 3e38 * 1e300
     assert torch.equal(torch.isnan(y).cpu(), nan) and torch.equal(y[:, 6:], x[:, 0, 6:])
+
+
+@pytest.mark.parametrize("norm", ["l2", "rms"])
+def test_head_norm_divides(ctx, norm):
+    """heads (a, 0, b, 0) of whole numbers whose length d is one: the norm is exact and each element is rounded once, as a division does it"""
+    m, n = np.meshgrid(np.arange(2, 60), np.arange(1, 59))
+    m, n = m[m > n], n[m > n]
+    keep = m * m + n * n < 4096                              # (d^2 < 2^24: the sum of squares is exact in f32)
+    m, n = m[keep], n[keep]
+    x = np.zeros((len(m), 1, 4))
+    x[:, 0, 0], x[:, 0, 2] = m * m - n * n, 2 * m * n
+    d = (m * m + n * n)[:, None, None] / (2.0 if norm == "rms" else 1.0)
+    y = _d(ctx.qk_norm_rope(torch.tensor(x, dtype=torch.float32, device=DEV), None, torch.zeros(len(m), 1, device=DEV),
+                            torch.zeros(0, dtype=torch.float64, device=DEV), (0,), norm=norm, eps=0.0)[0])
+    want = torch.tensor(x / d)
+    assert bool(((y - want).abs() <= HALF_STEP["f32"] * (1 + 2.0 ** -20) * want).all())
