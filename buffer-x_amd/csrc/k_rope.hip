@@ -174,14 +174,27 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeK p, int tpb)
         floats_of<T, N>(rb, b);
         if (row + RPB < nt * H) fetch(row + RPB);
         if (p.norm != BX_NORM_NONE) {
-            float sum = 0.0f;
+            const auto squares = [&]() __attribute__((always_inline)) {
+                float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
+                for (int i = 0; i < N; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
 #pragma unroll
-            for (int k = LPR / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, LPR);
+                for (int k = LPR / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, LPR);
+                return sum;
+            };
+            const bool rms = p.norm == BX_NORM_RMS;
+            float sum = squares(), eps = p.eps;
+            // squares out of f32's range: the head times a power of two, which x / d does not notice (small ones only where eps does not decide)
+            if (sum == INFINITY || (sum < 0x1p-80f && eps < (rms ? 0x1p-80f : 0x1p-40f))) {
+                const float s = sum == INFINITY ? 0x1p-70f : 0x1p90f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) { a[i] *= s; b[i] *= s; }
+                eps = rms ? eps * s * s : eps * s;
+                sum = squares();
+            }
             // x / d, by a product with 1 / d and what that leaves of x: as a division rounds it.  (A d that is zero or not finite has no such rest: d = 0
             // there makes it x, which counts for nothing.)
-            const float l2 = sqrtf(sum), d = p.norm == BX_NORM_RMS ? sqrtf(sum / (float)p.D + p.eps) : l2 < p.eps ? p.eps : l2, f = 1.0f / d;
+            const float l2 = sqrtf(sum), d = rms ? sqrtf(sum / (float)p.D + eps) : l2 < eps ? eps : l2, f = 1.0f / d;
             const bool safe = d > 0x1p-100f && d < 0x1p100f;
             const float dr = safe ? d : 0.0f, fr = safe ? f : 0.0f;
 #pragma unroll

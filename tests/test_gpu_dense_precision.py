@@ -181,3 +181,32 @@ def test_head_norm_divides(ctx, norm):
                             torch.zeros(0, dtype=torch.float64, device=DEV), (0,), norm=norm, eps=0.0)[0])
     want = torch.tensor(x / d)
     assert bool(((y - want).abs() <= HALF_STEP["f32"] * (1 + 2.0 ** -20) * want).all())
+
+
+@pytest.mark.parametrize("norm", ["l2", "rms"])
+@pytest.mark.parametrize("scale", [2.0 ** -110, 2.0 ** -60, 2.0 ** -30, 2.0 ** 55, 2.0 ** 63, 2.0 ** 100])
+def test_head_norm_far_from_one(ctx, norm, scale):
+    """what a head norm gives does not depend on a power of two in front of its elements, also where their squares leave f32's range"""
+    x = _rand(np.random.default_rng(1), (50, 3, 16), "f32")
+    args = (None, torch.zeros(50, 1, device=DEV), torch.zeros(0, dtype=torch.float64, device=DEV), (0,))
+    y = ctx.qk_norm_rope(x, *args, norm=norm, eps=0.0)[0]
+    got = ctx.qk_norm_rope(x * scale, *args, norm=norm, eps=0.0)[0]
+    assert bool(((got - y).abs() <= 2 * E * y.abs()).all()) and bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("norm", ["l2", "rms"])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("scale,eps", [(1e30, 1e-6), (1e25, 3e38), (1e-30, 1e-6), (1e-30, 1e-30), (1e-25, 0.0), (1e-38, 1e-37)])
+def test_head_norm_of_any_size(ctx, norm, dt, scale, eps):
+    """heads between large and small ones, with and without an eps that decides, against 64 bits: (D + 16) e of the factor and a division, the weight's
+    product and the result's rounding"""
+    D = 48
+    x = _rand(np.random.default_rng(2), (30, 2, D), "f32")
+    x[::3] *= scale
+    x = x.to(DT[dt])
+    w = _rand(np.random.default_rng(3), (D,), dt)
+    y = ctx.qk_norm_rope(x, None, torch.zeros(30, 1, device=DEV), torch.zeros(0, dtype=torch.float64, device=DEV), (0,), norm=norm, eps=eps, q_weight=w)[0]
+    X, e = _d(x), float(np.float32(eps))
+    d = torch.sqrt((X * X).mean(-1, keepdim=True) + e) if norm == "rms" else torch.clamp(X.norm(dim=-1, keepdim=True), min=e)
+    want = X / d * _d(w)
+    _within(y, want, HALF_STEP[dt] * want.abs() + (D + 20) * E * want.abs() * (1 + 2 * HALF_STEP[dt]) + TINY[dt])
