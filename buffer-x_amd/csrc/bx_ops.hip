@@ -17,15 +17,48 @@ bool misaligned(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(b
 // a stride that no memory can hold n of (this keeps every offset below inside 64 bits)
 bool bad_stride(long long s, long long n) { return s < 0 || (n > 1 && s > EXTENT_MAX / (n - 1)); }
 
-// the bytes that an operand's elements lie in, [lo, hi)
-struct Bytes { uintptr_t lo, hi; };
-Bytes span(const void* p, int e, long long n0, long long s0, long long n1 = 1, long long s1 = 0, long long n2 = 1, long long s2 = 0, long long n3 = 1)
+// an operand's elements: rows of `row` elements of `e` bytes at strides s (in elements) along up to three dimensions of sizes n
+struct Rows { const void* p; int e; long long row, n[3], s[3]; };
+Rows rows_of(const void* p, int e, long long row, long long n0 = 1, long long s0 = 0, long long n1 = 1, long long s1 = 0, long long n2 = 1, long long s2 = 0)
 {
-    if (!p || n0 <= 0 || n1 <= 0 || n2 <= 0 || n3 <= 0) return {0, 0};
-    const uintptr_t lo = (uintptr_t)p;
-    return {lo, lo + (uintptr_t)e * (uintptr_t)((n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + n3)};
+    return {p, e, row, {n0, n1, n2}, {s0, s1, s2}};
 }
-bool meet(Bytes a, Bytes b) { return a.lo < b.hi && b.lo < a.hi; }
+
+long long gcd(long long a, long long b) { while (b) { const long long t = a % b; a = b; b = t; } return a; }
+
+// Whether two operands may share memory.  They do not where the stretches that they lie in miss each other; nor where their rows are interleaved, as the
+// parts of one buffer are: with g the greatest common divisor of the strides along some dimensions of both, all rows of an operand lie at the same
+// place modulo g but for what the other dimensions add, and the two places have to miss each other.  Every choice of dimensions is tried.
+bool meet(const Rows& a, const Rows& b)
+{
+    const Rows* x[2] = {&a, &b};
+    long long extent[2];
+    for (int k = 0; k < 2; ++k) {
+        if (!x[k]->p || x[k]->row <= 0) return false;
+        extent[k] = x[k]->row;
+        for (int i = 0; i < 3; ++i) {
+            if (x[k]->n[i] <= 0) return false;
+            extent[k] += (x[k]->n[i] - 1) * x[k]->s[i];
+        }
+        extent[k] *= x[k]->e;
+    }
+    const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+    if (pa + (uintptr_t)extent[0] <= pb || pb + (uintptr_t)extent[1] <= pa) return false;
+    for (int mask = 1; mask < 64; ++mask) {
+        long long g = 0, in[2] = {a.row * a.e, b.row * b.e};
+        for (int k = 0; k < 2; ++k)
+            for (int i = 0; i < 3; ++i) {
+                if (x[k]->n[i] <= 1) continue;
+                const long long s = x[k]->s[i] * x[k]->e;
+                if (mask >> (3 * k + i) & 1) g = gcd(g, s);
+                else in[k] += (x[k]->n[i] - 1) * s;
+            }
+        if (g == 0 || in[0] > g || in[1] > g) continue;
+        const long long d = (long long)((pa > pb ? pa - pb : pb - pa) % (uintptr_t)g), at = pa >= pb || d == 0 ? d : g - d;      // a's place behind b's
+        if (at >= in[1] && at + in[0] <= g) return false;
+    }
+    return true;
+}
 
 // whether rows of n3 elements at strides s0, s1, s2 (sizes n0, n1, n2) share an element: dimensions are visited from the smallest stride
 // up, each has to clear what lies below it
@@ -43,24 +76,6 @@ bool self_overlap(long long n0, long long s0, long long n1, long long s1, long l
     return false;
 }
 
-// a head tensor [T][H][D] and another one: do they share an element?  Rows of one buffer (a projection that holds q and k side by side)
-// interleave without sharing any: their token strides are equal and the heads' stretches miss each other within it.
-struct Heads { const void* p; long long T, H, D, st, sh; };
-bool heads_meet(const Heads& a, const Heads& b, int e)
-{
-    if (!meet(span(a.p, e, a.T, a.st, a.H, a.sh, a.D > 0 ? 1 : 0, 0, a.D), span(b.p, e, b.T, b.st, b.H, b.sh, b.D > 0 ? 1 : 0, 0, b.D))) return false;
-    if (a.st != b.st) return true;
-    const long long ea = ((a.H - 1) * a.sh + a.D) * e, eb = ((b.H - 1) * b.sh + b.D) * e, st = a.st * e;
-    if (st < ea || st < eb) return true;
-    const long long d = (long long)((intptr_t)a.p - (intptr_t)b.p);
-    const long long delta = ((d % st) + st) % st;
-    return !(delta >= eb && delta + ea <= st);
-}
-bool same_heads(const Heads& a, const Heads& b)
-{
-    return a.p == b.p && (a.T <= 1 || a.st == b.st) && (a.H <= 1 || a.sh == b.sh);
-}
-
 int check_linear(const bx_linear_args* a)
 {
     OP_REFUSE(!a, "bx_linear: null argument");
@@ -76,10 +91,10 @@ int check_linear(const bx_linear_args* a)
     OP_REFUSE(a->M > 1 && a->ldy < a->N, "bx_linear: rows of y overlap (stride %lld, %lld columns)", (long long)a->ldy, (long long)a->N);
     OP_REFUSE(misaligned(a->x, e) || misaligned(a->w, e) || misaligned(a->bias, e) || misaligned(a->residual, e) || misaligned(a->y, e) ||
               misaligned(a->m_dev, 4), "bx_linear: a pointer is not aligned to its elements");
-    const Bytes y = span(a->y, e, a->M, a->ldy, 1, 0, 1, 0, a->N);
-    OP_REFUSE(meet(y, span(a->x, e, a->M, a->ldx, 1, 0, 1, 0, a->K)) || meet(y, span(a->w, e, a->N, a->ldw, 1, 0, 1, 0, a->K)) ||
-              meet(y, span(a->bias, e, 1, 0, 1, 0, 1, 0, a->N)) || meet(y, span(a->m_dev, 4, 1, 0)), "bx_linear: y overlaps an input");
-    OP_REFUSE(a->residual && !(a->residual == a->y && (a->M <= 1 || a->ldr == a->ldy)) && meet(y, span(a->residual, e, a->M, a->ldr, 1, 0, 1, 0, a->N)),
+    const Rows y = rows_of(a->y, e, a->N, a->M, a->ldy);
+    OP_REFUSE(meet(y, rows_of(a->x, e, a->K, a->M, a->ldx)) || meet(y, rows_of(a->w, e, a->K, a->N, a->ldw)) || meet(y, rows_of(a->bias, e, a->N)) ||
+              meet(y, rows_of(a->m_dev, 4, 1)), "bx_linear: y overlaps an input");
+    OP_REFUSE(a->residual && !(a->residual == a->y && (a->M <= 1 || a->ldr == a->ldy)) && meet(y, rows_of(a->residual, e, a->N, a->M, a->ldr)),
               "bx_linear: y overlaps the residual without being it");
     return BX_OK;
 }
@@ -113,20 +128,20 @@ int check_rope(const bx_qk_norm_rope_args* a)
     OP_REFUSE(misaligned(a->q, e) || misaligned(a->k, e) || misaligned(a->q_out, e) || misaligned(a->k_out, e) || misaligned(a->q_weight, e) ||
               misaligned(a->k_weight, e) || misaligned(a->pos, 4) || misaligned(a->freqs, 8) || misaligned(a->m_dev, 4),
               "bx_qk_norm_rope: a pointer is not aligned to its elements");
-    const Heads in[2] = {{has_q ? a->q : nullptr, a->T, a->Hq, a->D, a->q_stride_t, a->q_stride_h}, {has_k ? a->k : nullptr, a->T, a->Hk, a->D, a->k_stride_t, a->k_stride_h}};
-    const Heads out[2] = {{has_q ? a->q_out : nullptr, a->T, a->Hq, a->D, a->q_out_stride_t, a->q_out_stride_h},
-                          {has_k ? a->k_out : nullptr, a->T, a->Hk, a->D, a->k_out_stride_t, a->k_out_stride_h}};
+    const Rows in[2] = {rows_of(has_q ? a->q : nullptr, e, a->D, a->T, a->q_stride_t, a->Hq, a->q_stride_h),
+                        rows_of(has_k ? a->k : nullptr, e, a->D, a->T, a->k_stride_t, a->Hk, a->k_stride_h)};
+    const Rows out[2] = {rows_of(has_q ? a->q_out : nullptr, e, a->D, a->T, a->q_out_stride_t, a->Hq, a->q_out_stride_h),
+                         rows_of(has_k ? a->k_out : nullptr, e, a->D, a->T, a->k_out_stride_t, a->Hk, a->k_out_stride_h)};
+    const auto same = [](const Rows& x, const Rows& y) { return x.p == y.p && (x.n[0] <= 1 || x.s[0] == y.s[0]) && (x.n[1] <= 1 || x.s[1] == y.s[1]); };
     for (int i = 0; i < 2; ++i) {
-        if (!out[i].p) continue;
-        OP_REFUSE(self_overlap(out[i].T, out[i].st, out[i].H, out[i].sh, 1, 0, out[i].D), "bx_qk_norm_rope: rows of an output overlap");
-        const Bytes o = span(out[i].p, e, out[i].T, out[i].st, out[i].H, out[i].sh, 1, 0, a->D);
-        OP_REFUSE(meet(o, span(a->q_weight, e, 1, 0, 1, 0, 1, 0, a->D)) || meet(o, span(a->k_weight, e, 1, 0, 1, 0, 1, 0, a->D)) ||
-                  meet(o, span(a->pos, 4, a->T, a->pos_stride_t, 1, 0, 1, 0, a->axes)) || meet(o, span(a->freqs, 8, 1, 0, 1, 0, 1, 0, pairs)) ||
-                  meet(o, span(a->m_dev, 4, 1, 0)), "bx_qk_norm_rope: an output overlaps an input");
+        const Rows& o = out[i];
+        if (!o.p) continue;
+        OP_REFUSE(self_overlap(o.n[0], o.s[0], o.n[1], o.s[1], 1, 0, o.row), "bx_qk_norm_rope: rows of an output overlap");
+        OP_REFUSE(meet(o, rows_of(a->q_weight, e, a->D)) || meet(o, rows_of(a->k_weight, e, a->D)) || meet(o, rows_of(a->pos, 4, a->axes, a->T, a->pos_stride_t)) ||
+                  meet(o, rows_of(a->freqs, 8, pairs)) || meet(o, rows_of(a->m_dev, 4, 1)), "bx_qk_norm_rope: an output overlaps an input");
         for (int j = 0; j < 2; ++j) {
-            if (in[j].p && !(i == j && same_heads(out[i], in[j])))
-                OP_REFUSE(heads_meet(out[i], in[j], e), "bx_qk_norm_rope: an output overlaps an input without being it");
-            if (j > i && out[j].p) OP_REFUSE(heads_meet(out[i], out[j], e), "bx_qk_norm_rope: the outputs overlap");
+            OP_REFUSE(!(i == j && same(o, in[j])) && meet(o, in[j]), "bx_qk_norm_rope: an output overlaps an input without being it");
+            OP_REFUSE(j > i && meet(o, out[j]), "bx_qk_norm_rope: the outputs overlap");
         }
     }
     return BX_OK;
@@ -153,12 +168,12 @@ int check_attention(const bx_attention_args* a)
     OP_REFUSE(misaligned(a->q, e) || misaligned(a->k, e) || misaligned(a->v, e) || misaligned(a->o, e) || misaligned(a->q_lens, 4) ||
               misaligned(a->k_lens, 4) || misaligned(a->workspace, 16), "bx_attention: a pointer is not aligned to its elements (workspace: 16 bytes)");
     OP_REFUSE(self_overlap(a->B, a->o_stride_b, a->Lq, a->o_stride_t, a->Hq, a->o_stride_h, a->D), "bx_attention: rows of o overlap");
-    const Bytes o = span(a->o, e, a->B, a->o_stride_b, a->Lq, a->o_stride_t, a->Hq, a->o_stride_h, a->D);
-    const Bytes ws = span(a->workspace, 1, 1, 0, 1, 0, 1, 0, a->workspace_bytes);
-    const Bytes in[5] = {span(a->q, e, a->B, a->q_stride_b, a->Lq, a->q_stride_t, a->Hq, a->q_stride_h, a->D),
-                         span(a->k, e, a->B, a->k_stride_b, a->Lk, a->k_stride_t, a->Hk, a->k_stride_h, a->D),
-                         span(a->v, e, a->B, a->v_stride_b, a->Lk, a->v_stride_t, a->Hk, a->v_stride_h, a->D),
-                         span(a->q_lens, 4, a->B, 1), span(a->k_lens, 4, a->B, 1)};
+    const Rows o = rows_of(a->o, e, a->D, a->B, a->o_stride_b, a->Lq, a->o_stride_t, a->Hq, a->o_stride_h);
+    const Rows ws = rows_of(a->workspace, 1, a->workspace_bytes);
+    const Rows in[5] = {rows_of(a->q, e, a->D, a->B, a->q_stride_b, a->Lq, a->q_stride_t, a->Hq, a->q_stride_h),
+                        rows_of(a->k, e, a->D, a->B, a->k_stride_b, a->Lk, a->k_stride_t, a->Hk, a->k_stride_h),
+                        rows_of(a->v, e, a->D, a->B, a->v_stride_b, a->Lk, a->v_stride_t, a->Hk, a->v_stride_h),
+                        rows_of(a->q_lens, 4, a->B), rows_of(a->k_lens, 4, a->B)};
     OP_REFUSE(meet(o, ws), "bx_attention: o overlaps the workspace");
     for (int i = 0; i < 5; ++i) OP_REFUSE(meet(o, in[i]) || meet(ws, in[i]), "bx_attention: o or the workspace overlaps an input");
     return BX_OK;

@@ -310,7 +310,8 @@ int bx_refine(bx_ctx *ctx, void *stream, const float *ss, const float *tt, const
  * dimension is contiguous; a stride of 0 repeats a row), any element alignment is accepted and 16-byte aligned rows are faster.
  * Counts and lengths that depend on the data are device int32, read when the kernel runs and clamped to [0, the size given here];
  * rows at or behind them are neither read nor written.  Sizes of zero are answered without a launch.
- * Outputs must not overlap any input (exceptions are named) nor themselves: BX_ERR_ARG.  Results do not depend on the stream, on the
+ * Outputs must not share memory with any input (exceptions are named) nor their rows with each other: BX_ERR_ARG.  Rows that interleave, as
+ * parts of one buffer do, share none.  Results do not depend on the stream, on the
  * run or on other calls: the order of every sum is fixed by sizes, lengths and alignment.  The calls keep no state and share none, so several may run at
  * once, on one context too, and may be captured; the memory they are given must stay valid until they have run.  */
 #define BX_TYPE_F32 0
@@ -342,7 +343,7 @@ int bx_linear(bx_ctx *ctx, void *stream, const bx_linear_args *args);
  * with BX_PAIRS_HALF, (2 p, 2 p + 1) with BX_PAIRS_INTERLEAVED; elements from 2 P on are not rotated.
  * pos [T][axes] float32 or int32, freqs float64 [P] (radians per unit of position); t is their binary64 product, of any size (NaN where it
  * is not finite).  m_dev (nullable): device count of the tokens
- * in use.  q_out may be q itself and k_out k itself (same strides); interleaved rows of one buffer are not an overlap. */
+ * in use.  q_out may be q itself and k_out k itself (same strides). */
 #define BX_NORM_NONE 0
 #define BX_NORM_RMS 1
 #define BX_NORM_L2 2

@@ -210,3 +210,29 @@ def test_head_norm_of_any_size(ctx, norm, dt, scale, eps):
     d = torch.sqrt((X * X).mean(-1, keepdim=True) + e) if norm == "rms" else torch.clamp(X.norm(dim=-1, keepdim=True), min=e)
     want = X / d * _d(w)
     _within(y, want, HALF_STEP[dt] * want.abs() + (D + 20) * E * want.abs() * (1 + 2 * HALF_STEP[dt]) + TINY[dt])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(5, 64, 40), (700, 64, 40), (3000, 160, 333)])
+def test_linear_beside_its_input(ctx, dt, M, K, N):
+    """rows [x | y | residual] of one buffer: the same bits as apart, and nothing else is written"""
+    rng = np.random.default_rng(M)
+    rows = _rand(rng, (M, K + 2 * N + 3), dt)
+    x, y, r, rest = rows[:, :K], rows[:, K:K + N], rows[:, K + N:K + 2 * N], rows[:, K + 2 * N:]
+    w = _rand(rng, (N, K), dt, K ** -0.5)
+    want = ctx.linear(x, w, act="silu", residual=r)
+    before = rows.clone()
+    ctx.linear(x, w, act="silu", residual=r, out=y)
+    assert torch.equal(y, want) and torch.equal(x, before[:, :K]) and torch.equal(r, before[:, K + N:K + 2 * N]) and torch.equal(rest, before[:, K + 2 * N:])
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("L,D", [(1, 64), (300, 32), (300, 40), (200, 128)])
+def test_attention_beside_its_inputs(ctx, dt, L, D):
+    """rows [q | k | v | o] of one buffer"""
+    rows = _rand(np.random.default_rng(L + D), (2, L, 12, D), dt)
+    q, k, v, o = rows[:, :, :4], rows[:, :, 4:6], rows[:, :, 6:8], rows[:, :, 8:]
+    want = ctx.attention(q, k, v, window=(30, 0), sinks=2)
+    before = rows[:, :, :8].clone()
+    ctx.attention(q, k, v, window=(30, 0), sinks=2, out=o)
+    assert torch.equal(o, want) and torch.equal(rows[:, :, :8], before)
