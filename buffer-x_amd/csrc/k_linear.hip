@@ -5,11 +5,12 @@
 
 namespace {
 
-// Both activations go by |v| and the power 2^(-..) of it, so nothing overflows and small results keep their relative precision.
+// Both activations go by |v| and the power 2^(-..) of it, so nothing overflows and small results keep a relative precision.
 //   silu: v s (v >= 0) or v e s (v < 0),  e = exp(-|v|), s = 1 / (1 + e)
 //   gelu: v (1 - q) or v q,  q = Phi(-|v|) = exp(-v^2 / 2) t h(t),  t = 1 / (1 + 0.2625 |v|): h by the polynomial of degree 8 that fits
-//         0.5 erfcx(|v| / sqrt 2) / t with the least relative error (2e-8 over 0 .. 14.5).  20 instruction slots, where erfc takes over 50:
-//         at 67 million outputs that is a third of the time of the product itself.
+//         0.5 erfcx(|v| / sqrt 2) / t with the least relative error (3.4e-8 over 0 .. 14.5 with the coefficients as f32 has them; rounding v^2 in the
+//         exponent adds up to v^2 2^-24 of q).  20 instruction slots, where erfc takes over 50: at 67 million outputs that is a third of the time
+//         of the product itself.
 template <int act> __device__ __forceinline__ float act_of(float v)
 {
     if (act == BX_ACT_NONE) return v;
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(KS * WGM * WGN * 64) void linear_tile_kernel(Linear
 
 // f32 by bf16 planes: every operand is the sum of three bf16 numbers, a = a0 + a1 + a2 (8 + 8 + 8 bits, each the nearest to what is left: all 24
 // bits are there), taken apart on the way into LDS.  Six of the nine products are multiplied, the smallest first; the three left out are
-// below 2^-26 of a b, less than the rounding of one f32 product.  The six bf16 matrix instructions take 3/8 of the time of the f32 ones.
+// at most 2^-24 of |a b|, the rounding of one f32 product, and mostly far less (|a1| <= 2^-8 |a|, |a2| <= 2^-17 |a|).  The six bf16 matrix instructions take 3/8 of the time of the f32 ones.
 // An infinity leaves the planes as NaN: results that are not finite are summed again, in plain f32.
 template <int BM, int BN, int WGM, int WGN>
 __global__ __launch_bounds__(WGM * WGN * 64) void linear_planes_kernel(LinearK p)
