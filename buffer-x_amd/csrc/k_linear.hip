@@ -6,7 +6,7 @@
 namespace {
 
 // Both activations go by |v| and the power 2^(-..) of it, so nothing overflows and small results keep a relative precision.
-//   silu: v s (v >= 0) or v e s (v < 0),  e = exp(-|v|), s = 1 / (1 + e)
+//   silu: v s (v >= 0) or v h s h (v < 0),  h = exp(-|v| / 2), s = 1 / (1 + h^2): the power instruction ends at 2^-126, its square need not
 //   gelu: v (1 - q) or v q,  q = Phi(-|v|) = exp(-v^2 / 2) t h(t),  t = 1 / (1 + 0.2625 |v|): h by the polynomial of degree 8 that fits
 //         0.5 erfcx(|v| / sqrt 2) / t with the least relative error (3.4e-8 over 0 .. 14.5 with the coefficients as f32 has them; rounding v^2 in the
 //         exponent adds up to v^2 2^-24 of q).  20 instruction slots, where erfc takes over 50: at 67 million outputs that is a third of the time
@@ -16,8 +16,8 @@ template <int act> __device__ __forceinline__ float act_of(float v)
     if (act == BX_ACT_NONE) return v;
     if (act == BX_ACT_RELU) return v > 0.0f ? v : (v != v ? v : 0.0f);
     if (act == BX_ACT_SILU) {
-        const float e = __builtin_amdgcn_exp2f(fabsf(v) * -1.44269504f), s = __builtin_amdgcn_rcpf(1.0f + e);
-        return v * (v >= 0.0f ? s : e * s);
+        const float h = __builtin_amdgcn_exp2f(fabsf(v) * -0.72134752f), s = __builtin_amdgcn_rcpf(fmaf(h, h, 1.0f));
+        return v >= 0.0f ? v * s : v * h * s * h;
     }
     const float t = __builtin_amdgcn_rcpf(fmaf(0.2625f, fabsf(v), 1.0f));
     float h = 0.0305265988f;

@@ -236,3 +236,14 @@ def test_attention_beside_its_inputs(ctx, dt, L, D):
     before = rows[:, :, :8].clone()
     ctx.attention(q, k, v, window=(30, 0), sinks=2, out=o)
     assert torch.equal(o, want) and torch.equal(rows[:, :, :8], before)
+
+
+@pytest.mark.parametrize("M", [1, 70, 3000])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_silu_of_far_negative_numbers(ctx, M, dt):
+    """v / (1 + exp(-v)) down to the smallest normal numbers (v about -92), through products with one: the power's argument off by 2 e of itself and the
+    power by 4 e, twice, four products: (16 + 4 |v|) e"""
+    v = torch.linspace(-91, -60, M).to(DT[dt]).to(DEV)[:, None]
+    got = _d(ctx.linear(v, torch.ones((40, 1), dtype=DT[dt], device=DEV), act="silu"))
+    want = (_d(v) / (1 + torch.exp(-_d(v)))).expand(M, 40)
+    assert bool(((got - want).abs() <= (HALF_STEP[dt] + (16 + 4 * 91) * E) * want.abs() * (1 + HALF_STEP[dt]) + TINY[dt]).all())
