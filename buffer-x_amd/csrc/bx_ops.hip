@@ -215,7 +215,7 @@ int bx_qk_norm_rope(bx_ctx* c, void* stream, const bx_qk_norm_rope_args* a)
 int64_t bx_attention_workspace(bx_ctx* c, const bx_attention_args* a)
 {
     if (!c) { bx_set_error("null context"); return -1; }
-    if (!a || a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->Lk >= LEN_MAX || a->Hk < 1 || a->Hq < 1 || a->Hq % a->Hk != 0 || a->D < 1 || a->D > 128 ||
+    if (!a || a->dtype < BX_TYPE_F32 || a->dtype > BX_TYPE_BF16 || a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->Lk >= LEN_MAX || a->Hk < 1 || a->Hq < 1 || a->Hq % a->Hk != 0 || a->D < 1 || a->D > 128 ||
         a->sinks < 0 || (long long)a->B * a->Lq * a->Hq >= LEN_MAX || (long long)a->Lq * a->Hq >= LEN_MAX) {
         bx_set_error("bx_attention_workspace: bad argument");
         return -1;

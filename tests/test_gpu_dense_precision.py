@@ -247,3 +247,13 @@ def test_silu_of_far_negative_numbers(ctx, M, dt):
     got = _d(ctx.linear(v, torch.ones((40, 1), dtype=DT[dt], device=DEV), act="silu"))
     want = (_d(v) / (1 + torch.exp(-_d(v)))).expand(M, 40)
     assert bool(((got - want).abs() <= (HALF_STEP[dt] + (16 + 4 * 91) * E) * want.abs() * (1 + HALF_STEP[dt]) + TINY[dt]).all())
+
+
+def test_attention_workspace_of_no_type(ctx):
+    import ctypes as C
+    from bufferx_amd import dense
+    q, k, v = _attention_inputs("bf16", 1, 1, 9000, 2, 2, 64)
+    a, _ = dense.attention_args(torch, torch.device(DEV), q, k, v, None, (-1, -1), 0, None, None, None)
+    assert ctx.lib.bx_attention_workspace(ctx.handle, C.byref(a)) > 0
+    for a.dtype in (-1, 3):
+        assert ctx.lib.bx_attention_workspace(ctx.handle, C.byref(a)) == -1 and b"bad argument" in ctx.lib.bx_last_error()
