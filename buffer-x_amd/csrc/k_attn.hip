@@ -172,8 +172,8 @@ struct Rows {
     // the weights as second operands: registers of S^T as they are (f32), or as the sum of two (halves) or three (f32 by planes) numbers of the
     // operand's type, each the nearest to what the ones before it left.  Two hold 16 bits of bf16 weights and 22 of f16 ones; one alone loses as
     // much as the result's own rounding does (2-norm against 64 bits 2.28e-3 where rounding the result alone is 1.65e-3: 32768 positions of 16 / 4
-    // heads of 128, bf16, causal window of 1024 + 4).  The second product costs that case 328 -> 443 us, 1500 x 140 positions of 2 / 1 heads of
-    // 32, f16, a band of 49 + 1 32 -> 37 us, one query over 8192 keys 18.2 -> 18.8.
+    // heads of 128, bf16, causal window of 1024 + 4).  The second product costs that case 328 -> 438 us, 1500 x 140 positions of 2 / 1 heads of
+    // 32, f16, a band of 49 + 1 32 -> 36 us, one query over 8192 keys 18.2 -> 18.9.
     static constexpr int WP = NP == 3 ? 3 : 2;
     struct Weights { bxf16 s[sizeof(T) == 4 ? 2 : 1]; bxi4 f[WP][sizeof(T) == 4 ? 1 : 4]; };
     static constexpr int PLANE = BN * CPR;                   // chunks of a plane of K or V in LDS
@@ -303,11 +303,15 @@ struct Rows {
                 for (int j = 0; j < 8; ++j) e[j] = x.s[u / 2][8 * (u % 2) + j];
                 if constexpr (NP == 3) bx_planes(e, w.f[0][u], w.f[1][u], w.f[2][u]);
                 else {
-                    T hi[8], lo[8];
+                    // (in pairs: two numbers are rounded by one instruction, and widened again from what it leaves)
+                    typedef T t2 __attribute__((ext_vector_type(2)));
+                    t2 hi[4], lo[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        hi[j] = (T)e[j];
-                        lo[j] = (T)(e[j] - (float)hi[j]);
+                    for (int j = 0; j < 4; ++j) {
+                        unsigned pair = __builtin_bit_cast(unsigned, (t2){(T)e[2 * j], (T)e[2 * j + 1]});
+                        asm("" : "+v"(pair));
+                        hi[j] = __builtin_bit_cast(t2, pair);
+                        lo[j] = (t2){(T)(e[2 * j] - (float)hi[j][0]), (T)(e[2 * j + 1] - (float)hi[j][1])};
                     }
                     __builtin_memcpy(&w.f[0][u], hi, 16);
                     __builtin_memcpy(&w.f[1][u], lo, 16);
