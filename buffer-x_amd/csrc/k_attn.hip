@@ -10,6 +10,8 @@
 // V's first operand needs keys along the registers: halves are read from LDS with the transposing 8-byte load (lane group of 16 = 4 keys x 16
 // dimensions), floats one by one.
 //
+// (Times of halves that the comments below compare were taken with weights of one number each; two add 3 to 35 % to both sides.)
+//
 // Few rows, many keys: the key tiles are dealt to `nsplit` workgroups that leave (O, m, l) in the workspace and a second kernel
 // joins them in a fixed order.
 #include "bx_ops.h"
@@ -453,7 +455,7 @@ __device__ __forceinline__ void load8(const float* __restrict__ row, int k, int 
 constexpr int waves_of(int bytes, int DP, bool direct)
 {
     if (bytes == 4) return DP == 32 ? 3 : DP == 64 ? 2 : 1;
-    return DP == 128 ? 2 : (DP == 32 ? 4 : 3) - (direct ? 0 : 1);            // without spills in the loop
+    return DP == 128 ? 2 : (DP == 32 ? 4 : 3) - (direct ? 0 : 1);            // as many as fit without spills
 }
 template <class T, int DP, int NW, bool DIRECT>
 __global__ __launch_bounds__(NW * 64, waves_of(sizeof(T), DP, DIRECT)) void attn_kernel(AttnK p)

@@ -323,9 +323,9 @@ int bx_refine(bx_ctx *ctx, void *stream, const float *ss, const float *tt, const
 #define BX_ACT_SILU 3    /* v / (1 + exp(-v)) */
 
 /* y = act(x w^T + bias) + residual.  x [M][K], w [N][K], bias [N] (nullable), residual and y [M][N] (residual nullable; it may be y
- * itself, with the same stride).  M, N, K <= 2^30.  f32 sums of 128 terms and more run on the bf16 matrix units, every operand as three
- * bf16 numbers that hold all its 24 bits (operands below 2^-100 keep fewer); where an infinity or NaN is among them they are
- * summed again in plain f32.  m_dev (nullable): device count of the rows in use.                                               */
+ * itself, with the same stride).  M, N, K <= 2^30.  f32 sums of 128 terms and more may, depending on the sizes, run on the bf16 matrix
+ * units, every operand as three bf16 numbers that hold all its 24 bits (operands below 2^-100 keep fewer); results that meet an infinity or NaN there
+ * are summed again in plain f32, one after the other and slowly.  m_dev (nullable): device count of the rows in use.                                               */
 typedef struct bx_linear_args {
     int32_t dtype, act;
     int64_t M, N, K;
@@ -374,8 +374,8 @@ int bx_qk_norm_rope(bx_ctx *ctx, void *stream, const bx_qk_norm_rope_args *args)
  * does not see do not touch its result, whatever they hold, infinities and NaN included (the last place of it in one case, below).  scale in
  * [2^-100, 2^100].
  * q_lens / k_lens: device int32 [B], nullable (Lq / Lk).
- * Softmax weights are multiplied with 16 bits (bf16) or 22 (f16), not rounded to the type of v; f32 as in bx_linear.  Rows that meet an
- * infinity or NaN on the edge of their mask (f32: anywhere), or scores times scale of about 2^21 and more, are summed one by one with the 31 that
+ * Softmax weights are multiplied with 16 bits (bf16) or 22 (f16), not rounded to the type of v; f32 may run as in bx_linear.  Rows that meet an
+ * infinity or NaN on the edge of their mask (f32 by planes: anywhere), or scores times scale of about 3 million and more, are summed one by one with the 31 that
  * share a wave with them: right, but hundreds of times slower, and rounded differently in the last place.
  * workspace: device memory of bx_attention_workspace(ctx, args) bytes (0: none needed; a host function of the sizes alone), aligned to 16 bytes,
  * used until the call has run and by no other call meanwhile; BX_ERR_STATE when it is too small.               */
