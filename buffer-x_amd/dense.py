@@ -38,13 +38,14 @@ def _eager(torch):
     check that its operands need."""
     if not _STATE:
         from torch.autograd import forward_ad
-        _STATE.extend((torch._C._get_tracing_state, forward_ad))
-    if _STATE[0]() is not None:
+        _STATE.extend((torch.jit.is_tracing, forward_ad))
+    if _STATE[0]():
         raise ValueError("these operators cannot be traced (torch.jit.trace)")
     proxy = sys.modules.get("torch.fx.experimental.proxy_tensor")             # (not there: nobody traces with it)
     if proxy is not None and proxy.get_proxy_mode() is not None:
         raise ValueError("these operators cannot be traced (make_fx)")
-    return _operand if _STATE[1]._current_level < 0 else _checked            # (forward-mode derivatives are being taken somewhere)
+    # (a level of 0 and more: forward-mode derivatives are being taken)
+    return _operand if getattr(_STATE[1], "_current_level", 0) < 0 else _checked
 
 
 def _operand(torch, name, t, device, dtype, shape):
